@@ -111,6 +111,73 @@ SGQ_API int sgqd_embedding(const float* table, int64_t vocab, int64_t dim, const
  * a row of NaNs (or n == 0) gives 0. */
 SGQ_API int sgqd_argmax_rows(const float* x, int64_t rows, int64_t n, int64_t ld, int64_t* out, void* stream);
 
+/* ---- the INT8 key/value cache ------------------------------------------------------------------------------------
+ *
+ * Keys and values of a decoder block as INT8 codes with one fp32 scale per (sequence, kv head, position): head_dim + 4
+ * bytes per row in the place of 4 * head_dim.  A row r is held as sgq_quantize_int8 holds a row (SGQ_PER_ROW), bit for bit:
+ *   a = max(1e-8, max |r|),  scale = a / 127,  code = clamp(round_half_away(r * (127 / a)), -127, 127),
+ * all in fp32 (a NaN gets code +127; an infinity makes the scale infinite), and stands for code * scale.  Keys are rotated
+ * before they are quantized, every product and sum of the rotation rounded to fp32, so the codes depend on the inputs alone.
+ * The struct holds DEVICE pointers owned by the caller; it is read during the call only.  codes: [batch, n_kv_heads,
+ * max_seq, head_dim], 16-byte aligned; scales: [batch, n_kv_heads, max_seq].  Query head h reads kv head
+ * h / (n_heads / n_kv_heads).  `pos` is a DEVICE int32 per sequence (pos_stride 1) or one for all (pos_stride 0): the tokens
+ * of the sequence that are in the cache.  Rows of qkv are [n_heads | n_kv_heads | n_kv_heads] heads of head_dim values,
+ * qkv_stride floats apart; cos / sin tables as above, [table_rows, head_dim / 2], 16-byte aligned. */
+typedef struct sgqd_cache_int8 {
+    int8_t* k_codes;
+    float* k_scales;
+    int8_t* v_codes;
+    float* v_scales;
+    int64_t batch, n_kv_heads, max_seq, head_dim;
+} sgqd_cache_int8;
+
+/* t_new new tokens per sequence (row b * t_new + i of qkv: token i of sequence b, at position pos[b] + i): writes the rotated
+ * queries to q_out (rows q_stride floats apart; q_out == qkv with the same stride rotates in place, any other overlap is
+ * not allowed), and the rotated keys and the values, quantized, into the cache.  n_new (optional, DEVICE int32 per sequence):
+ * only the first n_new[b] tokens of sequence b exist (padded prompts).  rope_offset (optional, ONE DEVICE int32): added to
+ * the position for the rotation, for sequences behind a shared prefix.  table_rows >= max_seq.  A token that does not exist,
+ * whose position lies outside [0, max_seq) or whose rotation lies outside the tables changes nothing: no query and no row
+ * is written.
+ * head_dim: a multiple of 8, at most 256. */
+SGQ_API int sgqd_rope_kv_store_int8(const float* qkv, int64_t qkv_stride, int64_t t_new, int64_t n_heads, const float* cos_table,
+                                    const float* sin_table, int64_t table_rows, const int32_t* pos, int64_t pos_stride, const int32_t* n_new,
+                                    const int32_t* rope_offset, float* q_out, int64_t q_stride, const sgqd_cache_int8* cache,
+                                    void* stream);
+
+/* Reads positions [0, rows) back as fp32: k_out / v_out[b, h, out_row0 + t, :] = code * scale for b < batch, outputs
+ * [batch, n_kv_heads, out_max_seq, head_dim] (what the prompt attention takes as its caches).  A cache of one sequence
+ * (a shared prefix) is read into every one of `batch` sequences.  Other rows of the outputs are left as they were.
+ * head_dim: a multiple of 8, at most 256. */
+SGQ_API int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_t batch, float* k_out, float* v_out,
+                              int64_t out_max_seq, int64_t out_row0, void* stream);
+
+/* One decode step of attention for one NEW token per sequence (row b of qkv, position pos[b]): appends its rotated key and
+ * its value to the cache, quantized as above, and writes
+ *   out[b, h*head_dim + d] = sum_{t <= pos[b]} softmax_t(q_h . k_t / sqrt(head_dim)) v_t[d],
+ * k_t and v_t being the values the cache then holds, the new token's included.  qkv is read only.  A sequence whose pos lies
+ * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  A NaN or an infinity in a query
+ * gives NaN in its head's output, and so does a row with a scale that is not finite; rows at positions behind pos are not
+ * read.  The query and the softmax weights enter exact integer products as 24-bit fixed point (the query relative to its
+ * largest value, the weights relative to the largest of every 32 positions), sums are fp32: errors are those of an fp32
+ * evaluation.  table_rows >= max_seq.  head_dim must be 64 or 128.  prepared_out: as for sgqd_attn_decode. */
+SGQ_API int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,
+                                  const float* sin_table, int64_t table_rows, const int32_t* pos, int64_t pos_stride,
+                                  const sgqd_cache_int8* cache, float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes, void* stream);
+
+/* The same for sequences that begin with the same *prefix_len tokens (ONE DEVICE int32, taken as at least 0 and at most
+ * prefix->max_seq), whose rows lie once in `prefix`, a cache of one sequence with the same heads: every query attends to
+ * the prefix rows and to its own rows 0 .. pos[b], which stand at positions *prefix_len + t of its sequence (the rotation of
+ * the new token included; table_rows >= prefix->max_seq + max_seq).  The prefix is read once for the whole
+ * batch.  workspace: as many bytes as the query says (0: none), 256-byte aligned; it holds nothing from one call to the
+ * next, and calls that may run at the same time need one each. */
+SGQ_API size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                                            int64_t prefix_max);
+SGQ_API int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,
+                                         const float* sin_table, int64_t table_rows, const int32_t* pos,
+                                         int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix, const int32_t* prefix_len,
+                                         float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes, void* workspace,
+                                         size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -45,13 +45,20 @@ EXPORTS = [
 # every symbol include/sgq_decoder.h declares
 DECODER_EXPORTS = ["sgqd_add_rmsnorm", "sgqd_rope_kv_store", "sgqd_attn_decode", "sgqd_silu_mul", "sgqd_embedding",
                    "sgqd_argmax_rows", "sgqd_attn_prefill", "sgqd_attn_prefill_bf16", "sgqd_attn_decode_allgather",
-                   "sgqd_silu_mul_allgather"]
+                   "sgqd_silu_mul_allgather", "sgqd_rope_kv_store_int8", "sgqd_kv_load_int8", "sgqd_attn_decode_int8",
+                   "sgqd_attn_decode_prefix_int8", "sgqd_attn_decode_prefix_int8_workspace_bytes"]
 
 
 class SgqError(RuntimeError):
     def __init__(self, status: int, what: str, detail: str):
         super().__init__(f"{what}: {detail}" if detail else what)
         self.status = status
+
+
+class CacheInt8(C.Structure):
+    """sgqd_cache_int8 of include/sgq_decoder.h."""
+    _fields_ = [("k_codes", C.c_void_p), ("k_scales", C.c_void_p), ("v_codes", C.c_void_p), ("v_scales", C.c_void_p),
+                ("batch", C.c_int64), ("n_kv_heads", C.c_int64), ("max_seq", C.c_int64), ("head_dim", C.c_int64)]
 
 
 def _load() -> C.CDLL:
@@ -106,6 +113,13 @@ def _load() -> C.CDLL:
     lib.sgqd_attn_decode_allgather.argtypes = [p, i64, i64, i64, i64, p, p, p, p, i64, p, p, C.c_int, i64, i64, p]
     lib.sgqd_silu_mul_allgather.argtypes = [p, i64, i64, p, C.c_int, i64, i64, p]
     lib.sgqd_argmax_rows.argtypes = [p, i64, i64, i64, p, p]
+    cache = C.POINTER(CacheInt8)
+    lib.sgqd_rope_kv_store_int8.argtypes = [p, i64, i64, i64, p, p, i64, p, i64, p, p, p, i64, cache, p]
+    lib.sgqd_kv_load_int8.argtypes = [cache, i64, i64, p, p, i64, i64, p]
+    lib.sgqd_attn_decode_int8.argtypes = [p, i64, i64, p, p, i64, p, i64, cache, p, i64, p, sz, p]
+    lib.sgqd_attn_decode_prefix_int8.argtypes = [p, i64, i64, p, p, i64, p, i64, cache, cache, p, p, i64, p, sz, p, sz, p]
+    lib.sgqd_attn_decode_prefix_int8_workspace_bytes.restype = sz
+    lib.sgqd_attn_decode_prefix_int8_workspace_bytes.argtypes = [i64, i64, i64, i64, i64]
     return lib
 
 
@@ -304,6 +318,57 @@ def interleave_slices(gathered: torch.Tensor, world: int, M: int, n_local: int, 
     check(lib.sgq_interleave_slices(_ptr(gathered), world, M, n_local, _ptr(out), out.stride(0), _stream()),
           "sgq_interleave_slices")
     return out
+
+
+@dataclass
+class KVCacheInt8:
+    """Keys and values of one decoder block as INT8 codes [batch, kv_heads, max_seq, head_dim] with one fp32 scale per
+    (sequence, kv head, position): a row of head_dim values is held as quantize_int8(..., PER_ROW) holds it (the reference
+    has no cache: it recomputes every position, models.hpp:262-300)."""
+    k_codes: torch.Tensor
+    k_scales: torch.Tensor
+    v_codes: torch.Tensor
+    v_scales: torch.Tensor
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, max_seq: int, head_dim: int, device) -> "KVCacheInt8":
+        codes = [torch.zeros(batch, kv_heads, max_seq, head_dim, dtype=torch.int8, device=device) for _ in range(2)]
+        scales = [torch.zeros(batch, kv_heads, max_seq, device=device) for _ in range(2)]
+        return cls(codes[0], scales[0], codes[1], scales[1])
+
+
+def rope_kv_store_int8(qkv: torch.Tensor, cache: KVCacheInt8, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, n_heads: int, *,
+                       q_out: Optional[torch.Tensor] = None, rope_offset: Optional[torch.Tensor] = None,
+                       n_new: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """New tokens qkv[batch, tokens, (n_heads + 2 kv_heads) * head_dim]: token i of sequence b stands at position pos[b] + i
+    (pos: int32, one per sequence or one for all).  Rotates the queries into q_out (None: in place) and stores the rotated
+    keys and the values, quantized, in the cache.  n_new: tokens that exist per sequence, where prompts are padded;
+    rope_offset: positions in front of the cache (a shared prefix).  Tokens that do not exist or do not fit change nothing.
+    Returns q_out (or qkv)."""
+    return _native.rope_kv_store_int8(qkv, cache, cos, sin, pos, n_heads, q_out, rope_offset, n_new)
+
+
+def kv_load_int8(cache: KVCacheInt8, rows: int, *, batch: Optional[int] = None, k_out: Optional[torch.Tensor] = None,
+                 v_out: Optional[torch.Tensor] = None, row0: int = 0):
+    """Positions [0, rows) of the cache as the fp32 values they stand for, into rows row0 .. of k_out / v_out
+    [batch, kv_heads, max, head_dim] (None: new tensors of `rows` rows).  A cache of one sequence goes into each of `batch`."""
+    return _native.kv_load_int8(cache, rows, batch, k_out, v_out, row0)
+
+
+def attn_decode_int8(qkv: torch.Tensor, cache: KVCacheInt8, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, n_heads: int, *,
+                     out: Optional[torch.Tensor] = None, prepared: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One new token per sequence (qkv[batch, width], position pos[b]): appends it to the cache as rope_kv_store_int8 does and
+    returns its attention to positions 0 .. pos[b], [batch, n_heads * head_dim].  A sequence with pos outside the cache
+    takes no part (zeros).  prepared: also writes the output's prepared form (prepared_x_bytes), for linear_int4_prepared."""
+    return _native.attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared)
+
+
+def attn_decode_prefix_int8(qkv: torch.Tensor, cache: KVCacheInt8, prefix: KVCacheInt8, prefix_len: torch.Tensor, cos: torch.Tensor,
+                            sin: torch.Tensor, pos: torch.Tensor, n_heads: int, *, out: Optional[torch.Tensor] = None,
+                            prepared: Optional[torch.Tensor] = None, workspace: Optional[Workspace] = None) -> torch.Tensor:
+    """attn_decode_int8 for sequences that share their first prefix_len (one int32) tokens, held once in `prefix`, a cache of
+    one sequence: rows t of `cache` stand at positions prefix_len + t.  The prefix is read once for the whole batch."""
+    return _native.attn_decode_prefix_int8(qkv, cache, prefix, prefix_len, cos, sin, pos, n_heads, out, prepared, workspace)
 
 
 class QuantizedLinear:

@@ -18,7 +18,7 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 OBJ_DIR = os.path.join(HERE, "build")
 LIB = os.path.join(LIB_DIR, "libsgq.so")
-SOURCES = ["abi.cu", "quantize.cu", "linear_simt.cu", "gemv.cu", "gemm_tc.cu", "decoder_glue.cu", "peer.cu", "gemv_i8.cu", "linear_kn.cu"]
+SOURCES = ["abi.cu", "quantize.cu", "linear_simt.cu", "gemv.cu", "gemm_tc.cu", "decoder_glue.cu", "peer.cu", "gemv_i8.cu", "linear_kn.cu", "kv_int8.cu"]
 NVCC = os.environ.get("NVCC", "/usr/local/cuda/bin/nvcc")
 CUDA_HOME = os.environ.get("CUDA_HOME", "/usr/local/cuda")
 CXX = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
@@ -28,7 +28,7 @@ FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std
 
 def _deps(src: str) -> list[str]:
     hdrs = [os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith((".cuh", ".h"))]
-    return [src, os.path.join(os.path.dirname(HERE), "include", "sgq.h"), *hdrs]
+    return [src, *(os.path.join(os.path.dirname(HERE), "include", h) for h in ("sgq.h", "sgq_decoder.h")), *hdrs]
 
 
 def _stale(out: str, deps: list[str]) -> bool:
@@ -69,7 +69,7 @@ BINDING = os.path.join(LIB_DIR, "_sgq_torch.so")
 
 def build_binding(force: bool = False) -> str:
     """The Python package's native calls (csrc/torch_binding.cpp), against the installed torch's headers."""
-    if force or _stale(BINDING, [BINDING_SRC, os.path.join(os.path.dirname(HERE), "include", "sgq.h")]):
+    if force or _stale(BINDING, _deps(BINDING_SRC)):
         import sysconfig
 
         import torch

@@ -859,11 +859,8 @@ int launch_attn(const float* qkv, int64_t qkv_stride, int64_t batch, int n_heads
 
 using namespace sgq;
 
-extern "C" {
-
-namespace {
 // prepared_out is optional; when given, (rows, width) must have a prepared form and the buffer must hold it
-int check_prepared(void* prepared_out, size_t prepared_bytes, int64_t rows, int64_t width, PreparedLayout* L) {
+int sgq::check_prepared(void* prepared_out, size_t prepared_bytes, int64_t rows, int64_t width, PreparedLayout* L) {
     if (!prepared_out) return SGQ_OK;
     const size_t need = gemv_prepared_bytes(rows, width);
     if (need == 0) return bad(SGQ_ERR_UNSUPPORTED, "no prepared-activation form for this (rows, width): rows <= 16, width % 256 == 0");
@@ -871,7 +868,8 @@ int check_prepared(void* prepared_out, size_t prepared_bytes, int64_t rows, int6
     *L = prepared_layout(rows, width);
     return SGQ_OK;
 }
-}  // namespace
+
+extern "C" {
 
 int sgqd_add_rmsnorm(float* h, const float* delta, const float* gamma, float eps, int64_t rows, int64_t dim, float* out,
                      void* prepared_out, size_t prepared_bytes, void* stream) {

@@ -89,6 +89,9 @@ __host__ __device__ inline void digit_slot(int mode, int m, int j, int* set, int
     }
 }
 
+// Checks an operator's optional prepared output and gives its layout (decoder_glue.cu); SGQ_OK where there is none.
+int check_prepared(void* prepared_out, size_t prepared_bytes, int64_t rows, int64_t width, PreparedLayout* L);
+
 #ifdef __CUDACC__
 
 // Byte offset of the 8 fragment bytes of (group, set, fragment lane) inside the digit planes.

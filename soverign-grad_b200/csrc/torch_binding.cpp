@@ -12,6 +12,7 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -21,6 +22,7 @@
 #include <vector>
 
 #include "../../include/sgq.h"
+#include "../../include/sgq_decoder.h"
 
 namespace {
 
@@ -29,6 +31,7 @@ PyObject* g_tensor_class = nullptr;     // QuantizedTensor(qdata, scales, scheme
 PyObject* g_workspace_class = nullptr;  // Workspace: .buf, .get(nbytes)
 
 PyObject *s_qdata, *s_scales, *s_scheme, *s_shape, *s_group, *s_bits, *s_buf, *s_get;
+PyObject *s_k_codes, *s_k_scales, *s_v_codes, *s_v_scales;
 
 // A reference that is given back at the end of the scope.
 struct Ref {
@@ -345,6 +348,249 @@ PyObject* dequantize(PyObject* const* a, Py_ssize_t n) {
     return THPVariable_Wrap(std::move(out));
 }
 
+// ---- the INT8 key/value cache.  Every shape is checked before the device: the library sees pointers and sizes only. ----
+
+// A KVCacheInt8: k_codes / v_codes int8 [batch, kv heads, max_seq, head_dim], k_scales / v_scales fp32 [batch, kv heads, max_seq].
+struct Cache8 {
+    at::Tensor t[4];
+    sgqd_cache_int8 c = {};
+    explicit Cache8(PyObject* o) {
+        PyObject* names[4] = {s_k_codes, s_k_scales, s_v_codes, s_v_scales};
+        for (int i = 0; i < 4; ++i) {
+            Ref a(PyObject_GetAttr(o, names[i]));
+            if (!a) throw PythonError();
+            t[i] = as_tensor(a.p);
+        }
+        if (t[0].dim() != 4) raise(PyExc_RuntimeError, "cache codes must be [batch, kv heads, max_seq, head_dim]");
+        const auto rows = t[0].sizes().slice(0, 3);
+        for (int i = 0; i < 4; i += 2) {
+            if (t[i].scalar_type() != at::kChar || t[i].sizes() != t[0].sizes()) raise(PyExc_RuntimeError, "cache codes must be int8 of one shape");
+            if (t[i + 1].scalar_type() != at::kFloat || t[i + 1].sizes() != rows) raise(PyExc_RuntimeError, "cache scales must be fp32 [batch, kv heads, max_seq]");
+            if (!t[i].is_contiguous() || !t[i + 1].is_contiguous()) raise(PyExc_RuntimeError, "cache tensors must be contiguous");
+        }
+        c.batch = t[0].size(0); c.n_kv_heads = t[0].size(1); c.max_seq = t[0].size(2); c.head_dim = t[0].size(3);
+        if (c.n_kv_heads <= 0 || c.max_seq <= 0 || c.head_dim <= 0) raise(PyExc_RuntimeError, "the cache has no heads, positions or values");
+        c.k_codes = static_cast<int8_t*>(t[0].data_ptr()); c.k_scales = static_cast<float*>(t[1].data_ptr());
+        c.v_codes = static_cast<int8_t*>(t[2].data_ptr()); c.v_scales = static_cast<float*>(t[3].data_ptr());
+    }
+    void on(const c10::Device& d) const {
+        for (const at::Tensor& x : t)
+            if (x.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+    }
+};
+
+// Rows of `width` values spaced evenly: [batch, tokens, width], or [batch, width] where tokens may be 1.  stride < 0: they are not.
+struct Rows {
+    at::Tensor t;
+    int64_t batch, tokens, width, stride = -1;
+    explicit Rows(const at::Tensor& x, bool two) : t(x) {
+        if (t.dim() == 2 && two) t = t.unsqueeze(1);
+        if (t.dim() != 3) raise(PyExc_RuntimeError, two ? "rows must be [batch, width] or [batch, 1, width]" : "rows must be [batch, tokens, width]");
+        batch = t.size(0); tokens = t.size(1); width = t.size(2);
+        if (t.scalar_type() != at::kFloat || (t.stride(2) != 1 && width > 1)) return;
+        const int64_t step = tokens > 1 ? t.stride(1) : (batch > 1 ? t.stride(0) : width);
+        if (batch > 1 && tokens > 1 && t.stride(0) != tokens * step) return;
+        if (step < width || (step & 3) || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15)) return;
+        stride = step;
+    }
+};
+
+// Optional DEVICE int32 vector: nullptr for None
+struct Ints {
+    at::Tensor t;
+    const int32_t* p = nullptr;
+    int64_t n = 0;
+    Ints(PyObject* o, const char* what) {
+        if (o == Py_None) return;
+        t = as_tensor(o);
+        if (t.scalar_type() != at::kInt || t.dim() > 1 || (t.dim() == 1 && t.size(0) > 1 && t.stride(0) != 1)) raise(PyExc_RuntimeError, what);
+        n = t.numel();
+        p = static_cast<const int32_t*>(t.data_ptr());
+    }
+};
+
+// What the three calls that rotate have in common: qkv, tables, positions; all on one GPU.
+struct Rotary {
+    const Cache8& cache;
+    Rows qkv;
+    at::Tensor cos, sin;
+    Ints pos;
+    int64_t heads;
+    Rotary(PyObject* q, const Cache8& c, PyObject* cos_o, PyObject* sin_o, PyObject* pos_o, PyObject* heads_o, bool two)
+        : cache(c), qkv(as_tensor(q), two), cos(as_tensor(cos_o)), sin(as_tensor(sin_o)), pos(pos_o, "pos must be an int32 vector"),
+          heads(as_int(heads_o)) {
+        const int64_t hd = c.c.head_dim, kv = c.c.n_kv_heads;
+        if (heads <= 0 || heads % kv) raise(PyExc_RuntimeError, "n_heads must be a multiple of the cache's heads");
+        if (qkv.width != (heads + 2 * kv) * hd) raise(PyExc_RuntimeError, "qkv rows must hold n_heads + 2 * kv heads of head_dim values");
+        if (qkv.batch != c.c.batch) raise(PyExc_RuntimeError, "qkv and the cache differ in batch");
+        if (two && qkv.tokens != 1) raise(PyExc_RuntimeError, "one new token per sequence");
+        if (cos.dim() != 2 || cos.sizes() != sin.sizes() || cos.size(1) != hd / 2 || cos.scalar_type() != at::kFloat || sin.scalar_type() != at::kFloat ||
+            !cos.is_contiguous() || !sin.is_contiguous())
+            raise(PyExc_RuntimeError, "cos and sin must be fp32 [rows, head_dim / 2]");
+        if (!pos.p && pos.n == 0 && c.c.batch > 0) raise(PyExc_RuntimeError, "pos must be an int32 vector");
+        if (pos.n != 1 && pos.n != c.c.batch) raise(PyExc_RuntimeError, "pos must have one element, or one per sequence");
+        if (!qkv.t.is_cuda()) raise(PyExc_ValueError, "this library computes on CUDA tensors only");
+        const c10::Device d = qkv.t.device();
+        c.on(d);
+        if (cos.device() != d || sin.device() != d || pos.t.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+    }
+    int64_t pos_stride() const { return pos.n == 1 ? 0 : 1; }
+    // rows for reading: evenly spaced fp32, copied where they are not
+    void readable() {
+        if (qkv.stride < 0) qkv = Rows(qkv.t.to(at::kFloat).clone(at::MemoryFormat::Contiguous), false);
+    }
+};
+
+// rope_kv_store_int8(qkv, cache, cos, sin, pos, n_heads, q_out, rope_offset, n_new)
+PyObject* rope_kv_store_int8(PyObject* const* a, Py_ssize_t n) {
+    if (n != 9) raise(PyExc_TypeError, "rope_kv_store_int8 takes nine arguments");
+    const Cache8 cache(a[1]);
+    const bool in_place = a[6] == Py_None;
+    const at::Tensor q_out = in_place ? at::Tensor() : as_tensor(a[6]);
+    const Ints offset(a[7], "rope_offset must be one int32"), n_new(a[8], "n_new must be an int32 vector");
+    if (a[7] != Py_None && offset.n != 1) raise(PyExc_RuntimeError, "rope_offset must be one int32");
+    if (a[8] != Py_None && n_new.n != cache.c.batch) raise(PyExc_RuntimeError, "n_new must have one element per sequence");
+    Rotary r(a[0], cache, a[2], a[3], a[4], a[5], false);
+    const c10::Device d = r.qkv.t.device();
+    if ((offset.p && offset.t.device() != d) || (n_new.p && n_new.t.device() != d) || (!in_place && q_out.device() != d))
+        raise(PyExc_ValueError, "all tensors must be on one GPU");
+    const int64_t dim = r.heads * cache.c.head_dim;
+    if (in_place && r.qkv.stride < 0) raise(PyExc_RuntimeError, "in place, qkv must be evenly spaced fp32 rows aligned to 16 bytes");
+    const c10::cuda::CUDAGuard guard(d);
+    r.readable();
+    float* q_ptr = fptr(r.qkv.t);
+    int64_t q_stride = r.qkv.stride;
+    if (!in_place) {
+        const Rows q(q_out, false);
+        if (q.batch != r.qkv.batch || q.tokens != r.qkv.tokens || q.width != dim || q.stride < 0)
+            raise(PyExc_RuntimeError, "q_out must be evenly spaced fp32 rows [batch, tokens, n_heads * head_dim] aligned to 16 bytes");
+        q_ptr = fptr(q.t);
+        q_stride = q.stride;
+    }
+    void* s = stream();
+    check(without_gil([&] {
+              return sgqd_rope_kv_store_int8(fptr(r.qkv.t), r.qkv.stride, r.qkv.tokens, r.heads, fptr(r.cos), fptr(r.sin), r.cos.size(0), r.pos.p,
+                                             r.pos_stride(), n_new.p, offset.p, q_ptr, q_stride, &cache.c, s);
+          }),
+          "sgqd_rope_kv_store_int8");
+    PyObject* given = in_place ? a[0] : a[6];
+    Py_INCREF(given);
+    return given;
+}
+
+// kv_load_int8(cache, rows, batch, k_out, v_out, row0)
+PyObject* kv_load_int8(PyObject* const* a, Py_ssize_t n) {
+    if (n != 6) raise(PyExc_TypeError, "kv_load_int8 takes six arguments");
+    const Cache8 cache(a[0]);
+    const int64_t rows = as_int(a[1]), batch = a[2] == Py_None ? cache.c.batch : as_int(a[2]), row0 = as_int(a[5]);
+    if (rows < 0 || rows > cache.c.max_seq) raise(PyExc_RuntimeError, "rows must lie inside the cache");
+    if (batch < 0 || (batch != cache.c.batch && cache.c.batch != 1)) raise(PyExc_RuntimeError, "batch must be the cache's, or the cache one sequence");
+    if ((a[3] == Py_None) != (a[4] == Py_None)) raise(PyExc_RuntimeError, "give both outputs or neither");
+    if (row0 < 0 || (a[3] == Py_None && row0 != 0)) raise(PyExc_RuntimeError, "row0 goes with outputs of the caller's");
+    at::Tensor out[2];
+    int64_t out_rows = rows;
+    if (a[3] != Py_None) {
+        out[0] = as_tensor(a[3]);
+        out[1] = as_tensor(a[4]);
+        for (const at::Tensor& o : out) {
+            if (o.dim() != 4 || o.scalar_type() != at::kFloat || !o.is_contiguous() || o.sizes() != out[0].sizes() || o.size(0) != batch ||
+                o.size(1) != cache.c.n_kv_heads || o.size(3) != cache.c.head_dim || row0 > o.size(2) - rows)
+                raise(PyExc_RuntimeError, "outputs must be contiguous fp32 [batch, kv heads, row0 + rows or more, head_dim]");
+        }
+        out_rows = out[0].size(2);
+    }
+    const c10::Device d = cache.t[0].device();
+    if (!d.is_cuda()) raise(PyExc_ValueError, "this library computes on CUDA tensors only");
+    cache.on(d);
+    const c10::cuda::CUDAGuard guard(d);
+    if (a[3] == Py_None) {
+        for (at::Tensor& o : out) o = empty({batch, cache.c.n_kv_heads, rows, cache.c.head_dim}, at::kFloat, cache.t[0]);
+    } else if (out[0].device() != d || out[1].device() != d) {
+        raise(PyExc_ValueError, "all tensors must be on one GPU");
+    }
+    void* s = stream();
+    check(without_gil([&] { return sgqd_kv_load_int8(&cache.c, rows, batch, fptr(out[0]), fptr(out[1]), out_rows, row0, s); }), "sgqd_kv_load_int8");
+    return Py_BuildValue("(NN)", THPVariable_Wrap(out[0]), THPVariable_Wrap(out[1]));
+}
+
+// What the decode calls have in common behind the arguments `first` and `first + 1`: out, prepared
+struct DecodeOut {
+    at::Tensor out, planes;
+    PyObject* given;
+    int64_t stride;
+    uint8_t* p = nullptr;
+    size_t bytes = 0;
+    DecodeOut(PyObject* out_o, PyObject* planes_o, const Rotary& r) : given(out_o == Py_None ? nullptr : out_o) {
+        const int64_t batch = r.cache.c.batch, dim = r.heads * r.cache.c.head_dim;
+        const c10::Device d = r.qkv.t.device();
+        if (given) {
+            out = as_tensor(out_o);
+            if (out.dim() != 2 || out.size(0) != batch || out.size(1) != dim || out.scalar_type() != at::kFloat || out.stride(1) != 1 ||
+                (batch > 1 && out.stride(0) < dim))
+                raise(PyExc_RuntimeError, "out must be fp32 rows [batch, n_heads * head_dim]");
+            if (out.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+        }
+        if (planes_o != Py_None) {
+            planes = as_tensor(planes_o);
+            if (planes.scalar_type() != at::kByte || !planes.is_contiguous()) raise(PyExc_RuntimeError, "prepared must be a uint8 buffer");
+            if (planes.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+            p = static_cast<uint8_t*>(planes.data_ptr());
+            bytes = static_cast<size_t>(planes.numel());
+        }
+        if (!given) out = empty({batch, dim}, at::kFloat, r.qkv.t);
+        stride = batch > 1 ? out.stride(0) : dim;
+    }
+    PyObject* result() {
+        if (!given) return THPVariable_Wrap(std::move(out));
+        Py_INCREF(given);
+        return given;
+    }
+};
+
+// attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared)
+PyObject* attn_decode_int8(PyObject* const* a, Py_ssize_t n) {
+    if (n != 8) raise(PyExc_TypeError, "attn_decode_int8 takes eight arguments");
+    const Cache8 cache(a[1]);
+    Rotary r(a[0], cache, a[2], a[3], a[4], a[5], true);
+    const c10::cuda::CUDAGuard guard(r.qkv.t.device());
+    r.readable();
+    DecodeOut o(a[6], a[7], r);
+    void* s = stream();
+    check(without_gil([&] {
+              return sgqd_attn_decode_int8(fptr(r.qkv.t), r.qkv.stride, r.heads, fptr(r.cos), fptr(r.sin), r.cos.size(0), r.pos.p, r.pos_stride(), &cache.c,
+                                           fptr(o.out), o.stride, o.p, o.bytes, s);
+          }),
+          "sgqd_attn_decode_int8");
+    return o.result();
+}
+
+// attn_decode_prefix_int8(qkv, cache, prefix, prefix_len, cos, sin, pos, n_heads, out, prepared, workspace)
+PyObject* attn_decode_prefix_int8(PyObject* const* a, Py_ssize_t n) {
+    if (n != 11) raise(PyExc_TypeError, "attn_decode_prefix_int8 takes eleven arguments");
+    const Cache8 cache(a[1]), prefix(a[2]);
+    const Ints len(a[3], "prefix_len must be one int32");
+    if (len.n != 1) raise(PyExc_RuntimeError, "prefix_len must be one int32");
+    if (prefix.c.batch != 1 || prefix.c.n_kv_heads != cache.c.n_kv_heads || prefix.c.head_dim != cache.c.head_dim)
+        raise(PyExc_RuntimeError, "the prefix is one sequence with the cache's heads");
+    Rotary r(a[0], cache, a[4], a[5], a[6], a[7], true);
+    const c10::Device d = r.qkv.t.device();
+    prefix.on(d);
+    if (len.t.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+    const c10::cuda::CUDAGuard guard(d);
+    r.readable();
+    DecodeOut o(a[8], a[9], r);
+    const Scratch ws(a[10], sgqd_attn_decode_prefix_int8_workspace_bytes(cache.c.batch, r.heads, cache.c.n_kv_heads, cache.c.head_dim, prefix.c.max_seq),
+                     r.qkv.t);
+    if (ws.buf.defined() && ws.buf.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
+    void* s = stream();
+    check(without_gil([&] {
+              return sgqd_attn_decode_prefix_int8(fptr(r.qkv.t), r.qkv.stride, r.heads, fptr(r.cos), fptr(r.sin), r.cos.size(0), r.pos.p, r.pos_stride(),
+                                                  &cache.c, &prefix.c, len.p, fptr(o.out), o.stride, o.p, o.bytes, ws.ptr, ws.bytes, s);
+          }),
+          "sgqd_attn_decode_prefix_int8");
+    return o.result();
+}
+
 // set_classes(SgqError, QuantizedTensor, Workspace)
 PyObject* set_classes(PyObject* const* a, Py_ssize_t n) {
     if (n != 3) raise(PyExc_TypeError, "set_classes takes three arguments");
@@ -360,7 +606,8 @@ PyObject* set_classes(PyObject* const* a, Py_ssize_t n) {
 #define SGQ_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&entry<name>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {
     SGQ_METHOD(quantized_matmul), SGQ_METHOD(backward_x), SGQ_METHOD(linear_w8a8), SGQ_METHOD(quantize_int8),
-    SGQ_METHOD(quantize_int4),    SGQ_METHOD(dequantize), SGQ_METHOD(set_classes), {nullptr, nullptr, 0, nullptr}};
+    SGQ_METHOD(quantize_int4),    SGQ_METHOD(dequantize), SGQ_METHOD(rope_kv_store_int8), SGQ_METHOD(kv_load_int8),
+    SGQ_METHOD(attn_decode_int8), SGQ_METHOD(attn_decode_prefix_int8), SGQ_METHOD(set_classes), {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_sgq_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 
@@ -375,5 +622,9 @@ PyMODINIT_FUNC PyInit__sgq_torch(void) {
     s_bits = PyUnicode_InternFromString("bits");
     s_buf = PyUnicode_InternFromString("buf");
     s_get = PyUnicode_InternFromString("get");
+    s_k_codes = PyUnicode_InternFromString("k_codes");
+    s_k_scales = PyUnicode_InternFromString("k_scales");
+    s_v_codes = PyUnicode_InternFromString("v_codes");
+    s_v_scales = PyUnicode_InternFromString("v_scales");
     return PyModule_Create(&g_module);
 }
