@@ -11,6 +11,7 @@
 
 #include "../../include/sgq_decoder.h"
 
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 namespace sgq {
@@ -18,6 +19,7 @@ namespace sgq {
 namespace {
 
 constexpr int kMaxHeadDim = 256;
+constexpr int64_t kMaxPositions = 1ll << 30;       // of the attention: positions and strides between tiles in 32 bits
 
 // (x1, x2) of a rotary pair, every operation rounded (src/ops.cpp:1737-1738)
 __device__ __forceinline__ void rotate_pair(float& x1, float& x2, float c, float s) {
@@ -124,6 +126,23 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t
 }
 
 // ---- decode attention -------------------------------------------------------------------------------------------------
+// Both products of the attention run on the tensor cores as exact integer products (mma.sync m16n8k32, s8 x s8 -> s32): the
+// codes go in as they lie in memory, the query and the softmax weights as 24-bit fixed point split into three balanced
+// base-256 digits (the arithmetic of gemv_prepare.cuh), one digit per column of the small operand.
+//
+//   scores   A = 16 rows of the cache x 32 values, B = 32 values x 8 columns.  A lane (g, t) = (lane / 4, lane % 4) of the
+//            warp loads the 16-byte chunks t (and 4 + t) of the rows 4g .. 4g+3 of a tile of 32 positions: these ARE the A
+//            fragments, the order of the head dimension inside them being the same in the query's digits.  Columns 2t, 2t+1
+//            of a "main" column set hold digits 2 and 1 of query t, those of the "low" set digit 0 of queries t and
+//            t + 4, so a lane finds all digits of its one or two queries in its own accumulators.
+//   weights  w = p * value scale, relative to the largest |w| of the tile and query: their digits cross the warp by shuffles
+//            (rows of the accumulators become the contraction index).
+//   output   A = 16 values x 32 positions: a lane loads HD/8 consecutive values of 8 positions and transposes 4 x 4 bytes
+//            with byte permutes.  B = 32 positions x 8 columns of weight digits.
+//
+// Scores and outputs leave the integer domain once per tile (sum of 32 or HD products below 2^22, exact as fp32), scaled
+// and added in fp32 with the running maximum and sum of the softmax.  A lane holds the scores of positions 4g .. 4g+3 and
+// the values [HD/8 g, HD/8 (g+1)) of the outputs of queries t and t + 4.
 struct CacheView {
     int8_t* kc;
     float* ks;
@@ -132,98 +151,507 @@ struct CacheView {
     int64_t max_seq;
 };
 
-// One block per (sequence, kv head).  The block appends the new token's row, then its warps walk the positions (the prefix's,
-// then the sequence's own) with a running maximum and sum, one query head after the other.
-constexpr int kSimpleWarps = 8;
+// D = A(16x32, s8) * B(32x8, s8) + magic (see gemv_prepare.cuh: the sum read as fp32 bits is 12582912 + S), and D += A * B
+__device__ __forceinline__ void mma_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kMagicBits));
+}
+__device__ __forceinline__ void mma_next(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// digit sums (2: highest) of one exact sum, as fp32
+__device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
+    const float f2 = __int_as_float(d2) - kMagicF, f1 = __int_as_float(d1) - kMagicF, f0 = __int_as_float(d0) - kMagicF;
+    return fmaf(f2, 65536.0f, fmaf(f1, 256.0f, f0));
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+constexpr int kTile = 32;              // positions per step of a warp
+
+// One warp's running attention of up to NQ (4 or 8) queries over tiles of one kv head's rows.
+template <int HD, int NQ>
+struct WarpAttention {
+    static constexpr int KW = HD / 16;         // 32-bit words of a key row per lane
+    static constexpr int VB = HD / 8;          // values per lane and position
+    static constexpr int VW = VB / 4;
+    static constexpr int NS = NQ / 4, NT = NS + 1;
+    static constexpr int kQueryBytes = 3 * HD; // digit planes of one query: [digit][HD]
+
+    uint32_t k[4][KW], v[8][VW], bq[NT][KW];
+    float ks[4], vs[4];
+    float qu[NS], m[NS], l[NS], o[NS][VB];
+    int g, t;
+
+    __device__ __forceinline__ void init(int lane) {
+        g = lane >> 2;
+        t = lane & 3;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            m[s] = -CUDART_INF_F;
+            l[s] = 0.f;
+#pragma unroll
+            for (int j = 0; j < VB; ++j) o[s][j] = 0.f;
+        }
+    }
+    // the digit planes and units of NQ queries, written by query_digits below
+    __device__ __forceinline__ void load_queries(const uint8_t* planes, const float* units) {
+        auto rd = [&](uint32_t (&w)[KW], int query, int digit, bool zero) {
+            const uint8_t* p = planes + query * kQueryBytes + digit * HD + 16 * t;
+#pragma unroll
+            for (int c = 0; c < KW / 4; ++c) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p + 64 * c);
+                w[4 * c] = zero ? 0u : x.x; w[4 * c + 1] = zero ? 0u : x.y; w[4 * c + 2] = zero ? 0u : x.z; w[4 * c + 3] = zero ? 0u : x.w;
+            }
+        };
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            rd(bq[s], 4 * s + (g >> 1), 2 - (g & 1), false);
+            qu[s] = units[4 * s + t];
+        }
+        if (NS == 2) rd(bq[NS], (g >> 1) + 4 * (g & 1), 0, false);
+        else rd(bq[NS], g >> 1, 0, (g & 1) != 0);
+    }
+    __device__ __forceinline__ void load_k(const int8_t* kc, const float* ksc, int t0, int t1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int key = t0 + 4 * g + i;
+            key = key < t1 ? key : t1 - 1;                    // clamped: masked in step()
+            const uint4* p = reinterpret_cast<const uint4*>(kc + static_cast<int64_t>(key) * HD + 16 * t);
+#pragma unroll
+            for (int c = 0; c < KW / 4; ++c) {
+                const uint4 x = p[4 * c];
+                k[i][4 * c] = x.x; k[i][4 * c + 1] = x.y; k[i][4 * c + 2] = x.z; k[i][4 * c + 3] = x.w;
+            }
+            ks[i] = ksc[key];
+        }
+    }
+    __device__ __forceinline__ void load_v(const int8_t* vc, const float* vsc, int t0, int t1) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            int key = t0 + 4 * g + i;
+            key = key < t1 ? key : t1 - 1;
+            vs[i] = vsc[key];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            int key = t0 + 4 * t + (i & 3) + 16 * (i >> 2);
+            key = key < t1 ? key : t1 - 1;
+            const int8_t* p = vc + static_cast<int64_t>(key) * HD + VB * g;
+            if constexpr (VW == 4) {
+                const uint4 x = *reinterpret_cast<const uint4*>(p);
+                v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+            } else {
+                const uint2 x = *reinterpret_cast<const uint2*>(p);
+                v[i][0] = x.x; v[i][1] = x.y;
+            }
+        }
+    }
+    // scores of the loaded keys: sc[s][i] of position t0 + 4g + i and query t + 4s, in base-2 units
+    __device__ __forceinline__ void scores(float (&sc)[NS][4], int t0, int t1) {
+        int acc[2][NT][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                mma_first(acc[h][n], k[2 * h][0], k[2 * h + 1][0], k[2 * h][1], k[2 * h + 1][1], bq[n][0], bq[n][1]);
+#pragma unroll
+                for (int c = 1; c < KW / 2; ++c)
+                    mma_next(acc[h][n], k[2 * h][2 * c], k[2 * h + 1][2 * c], k[2 * h][2 * c + 1], k[2 * h + 1][2 * c + 1], bq[n][2 * c], bq[n][2 * c + 1]);
+            }
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int h = i >> 1, r = 2 * (i & 1);
+                const float x = join_digits(acc[h][s][r], acc[h][s][r + 1], acc[h][NS][r + s]) * qu[s];
+                const float y = fmaf(x, ks[i], ks[i] - ks[i]);          // NaN for a row whose scale is not finite
+                sc[s][i] = t0 + 4 * g + i < t1 ? y : -CUDART_INF_F;
+            }
+    }
+    // the tile's weights into the running softmax, and its values into the outputs
+    __device__ __forceinline__ void accumulate(float (&sc)[NS][4], int t0, int t1) {
+        uint32_t bw[NT][2];
+        float corr[NS], unit[NS];
+        uint32_t w0[NS], w1[NS], w2[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            float top = fmaxf(fmaxf(sc[s][0], sc[s][1]), fmaxf(sc[s][2], sc[s][3]));
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+            const float mn = fmaxf(m[s], top);
+            corr[s] = m[s] == mn ? 1.0f : exp2_approx(m[s] - mn);
+            m[s] = mn;
+            float w[4], sum = 0.f, most = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float p = sc[s][i] == -CUDART_INF_F ? 0.f : exp2_approx(sc[s][i] - mn);
+                sum += p;
+                w[i] = p * (t0 + 4 * g + i < t1 ? vs[i] : 0.f);
+                most = max_nan(most, fabsf(w[i]));
+            }
+            l[s] = fmaf(l[s], corr[s], sum);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
+            // a tile whose weights vanish against the running maximum contributes nothing; NaN and infinity pass
+            const float per = most < 1e-30f ? 0.f : __fdividef(kDigitRange, most);
+            unit[s] = most * (1.0f / kDigitRange);
+            uint32_t d[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) d[i] = digit_bytes(__float2int_rn(w[i] * per));
+            const uint32_t x = __byte_perm(d[0], d[1], 0x5140), y = __byte_perm(d[2], d[3], 0x5140);
+            w0[s] = __byte_perm(x, y, 0x5410);
+            w1[s] = __byte_perm(x, y, 0x7632);
+            w2[s] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+        }
+        // B fragments: lane (column g, position quad t or t + 4) takes the digit words that lane (quad, query) holds
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const int from = 4 * (t + 4 * half) + (g >> 1);
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                const uint32_t hi = __shfl_sync(0xffffffffu, w2[s], from), mid = __shfl_sync(0xffffffffu, w1[s], from);
+                bw[s][half] = (g & 1) ? mid : hi;
+            }
+            const uint32_t lo = __shfl_sync(0xffffffffu, w0[0], from);
+            const uint32_t lo2 = NS == 2 ? __shfl_sync(0xffffffffu, w0[NS - 1], from) : 0u;
+            bw[NS][half] = (g & 1) ? lo2 : lo;
+        }
+#pragma unroll
+        for (int wd = 0; wd < VW; ++wd) {
+            uint32_t a[2][4];                   // [quad half][value 4 wd + r]: four positions each
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t x0 = v[4 * q][wd], x1 = v[4 * q + 1][wd], x2 = v[4 * q + 2][wd], x3 = v[4 * q + 3][wd];
+                const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
+                const uint32_t p2 = __byte_perm(x2, x3, 0x5140), p3 = __byte_perm(x2, x3, 0x7362);
+                a[q][0] = __byte_perm(p0, p2, 0x5410);
+                a[q][1] = __byte_perm(p0, p2, 0x7632);
+                a[q][2] = __byte_perm(p1, p3, 0x5410);
+                a[q][3] = __byte_perm(p1, p3, 0x7632);
+            }
+#pragma unroll
+            for (int pr = 0; pr < 2; ++pr) {    // values 4 wd + 2 pr (rows g) and 4 wd + 2 pr + 1 (rows g + 8)
+                int acc[NT][4];
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma_first(acc[n], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[n][0], bw[n][1]);
+#pragma unroll
+                for (int s = 0; s < NS; ++s)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        float& out = o[s][4 * wd + 2 * pr + e];
+                        out = fmaf(out, corr[s], join_digits(acc[s][2 * e], acc[s][2 * e + 1], acc[NS][2 * e + s]) * unit[s]);
+                    }
+            }
+        }
+    }
+    // tiles t0, t0 + stride, ... below t1 of the rows at kc / vc; the first one's loads may be under way (`loaded`)
+    __device__ __forceinline__ void run(const int8_t* kc, const float* ksc, const int8_t* vc, const float* vsc, int t0, int t1, int stride) {
+        for (; t0 < t1; t0 += stride) {
+            float sc[NS][4];
+            scores(sc, t0, t1);
+            const bool more = t1 - t0 > stride;
+            if (more) load_k(kc, ksc, t0 + stride, t1);       // on their way while this tile's values are added up
+            accumulate(sc, t0, t1);
+            if (more) load_v(vc, vsc, t0 + stride, t1);
+        }
+    }
+    // (max, sum, value) of every query into sm_ml[NQ][2], sm_o[NQ][HD]
+    __device__ __forceinline__ void store(float* sm_ml, float* sm_o) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) l[s] += __shfl_xor_sync(0xffffffffu, l[s], d);
+            const int q = t + 4 * s;
+            if (g == 0) { sm_ml[2 * q] = m[s]; sm_ml[2 * q + 1] = l[s]; }
+#pragma unroll
+            for (int j = 0; j < VB; j += 4)
+                *reinterpret_cast<float4*>(sm_o + q * HD + VB * g + j) = make_float4(o[s][j], o[s][j + 1], o[s][j + 2], o[s][j + 3]);
+        }
+    }
+};
+
+// One warp, one row of HD values (VEC consecutive per lane), rotated if `turn`.
 template <int HD>
-__global__ void __launch_bounds__(kSimpleWarps * 32) attn_decode_int8_kernel(const float* __restrict__ qkv, int64_t qkv_stride, int n_heads, int n_kv,
-                                                                             const float* __restrict__ cos_t, const float* __restrict__ sin_t,
-                                                                             const int32_t* __restrict__ pos_p, int64_t pos_stride, CacheView own,
-                                                                             CacheView first, const int32_t* __restrict__ prefix_len,
-                                                                             float* __restrict__ out, int64_t out_stride) {
+__device__ __forceinline__ void load_row(float (&v)[HD / 32], const float* row, const float* cos_row, const float* sin_row, bool turn, int lane) {
     constexpr int VEC = HD / 32;
-    __shared__ float sm_m[kSimpleWarps], sm_l[kSimpleWarps], sm_acc[kSimpleWarps][HD];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) v[j] = row[lane * VEC + j];
+    if (!turn) return;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
+        const float c = cos_row[(lane & 15) * VEC + j], s = sin_row[(lane & 15) * VEC + j];
+        float x1 = lane < 16 ? v[j] : other, x2 = lane < 16 ? other : v[j];
+        rotate_pair(x1, x2, c, s);
+        v[j] = lane < 16 ? x1 : x2;
+    }
+}
+
+// The rotated query as digit planes [3][HD] and its unit, which carries 1/sqrt(HD) and log2(e).  A NaN or an infinity in the
+// query makes the unit NaN or infinite and the digits zero: every score is NaN.
+template <int HD>
+__device__ __forceinline__ void query_digits(const float (&v)[HD / 32], uint8_t* planes, float* unit, int lane) {
+    constexpr int VEC = HD / 32;
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    top = __reduce_max_sync(0xffffffffu, top);
+    const float most = __uint_as_float(top);
+    const bool fine = top < 0x7F800000u && most >= 1e-30f;
+    const float per = fine ? __fdiv_rn(kDigitRange, most) : 0.f;
+    uint32_t d[VEC];
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) d[j] = fine ? digit_bytes(__float2int_rn(__fmul_rn(v[j], per))) : 0u;
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+        if constexpr (VEC == 4)
+            *reinterpret_cast<uint32_t*>(planes + j * HD + lane * 4) = gather_byte(d[0], d[1], d[2], d[3], j);
+        else
+            *reinterpret_cast<uint16_t*>(planes + j * HD + lane * 2) = static_cast<uint16_t>(__byte_perm(d[0], d[1], 0x0040 + 0x11 * j));
+    }
+    if (lane == 0) *unit = top >= 0x7F800000u ? CUDART_NAN_F : (fine ? __fmul_rn(__fdiv_rn(most, kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f);
+}
+
+// One warp quantizes a row into the cache.
+template <int HD>
+__device__ __forceinline__ void append_row(const float (&v)[HD / 32], int8_t* codes, float* scale, int lane) {
+    constexpr int VEC = HD / 32;
+    float top = 1e-8f;
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) top = absmax_step(top, v[j]);
+    top = warp_max(top);
+    const float inv = __fdiv_rn(127.0f, top);
+    if constexpr (VEC == 4)
+        *reinterpret_cast<char4*>(codes + lane * 4) = make_char4(quantize_code<127, -127>(v[0], inv), quantize_code<127, -127>(v[1], inv),
+                                                                 quantize_code<127, -127>(v[2], inv), quantize_code<127, -127>(v[3], inv));
+    else
+        *reinterpret_cast<char2*>(codes + lane * 2) = make_char2(quantize_code<127, -127>(v[0], inv), quantize_code<127, -127>(v[1], inv));
+    if (lane == 0) *scale = __fdiv_rn(top, 127.0f);
+}
+
+struct DecodeArgs {
+    const float* qkv;
+    int64_t qkv_stride;
+    int n_heads, n_kv, batch;
+    const float* cos_t;
+    const float* sin_t;
+    const int32_t* pos;
+    int64_t pos_stride;
+    CacheView own, first;              // first: the shared prefix (prefix_len != NULL)
+    const int32_t* prefix_len;
+    float* out;
+    int64_t out_stride;
+    int pmode, nmain, nlow;
+    uint8_t* planes;
+    const float* part_ml;              // prefix partial results [kv head][row][split][2] and [...][HD]
+    const float* part_o;
+    int parts;
+};
+
+__device__ __forceinline__ int64_t prefix_rows(const DecodeArgs& a) {
+    if (!a.prefix_len) return 0;
+    const int64_t p = *a.prefix_len;
+    return p < 0 ? 0 : (p > a.first.max_seq ? a.first.max_seq : p);
+}
+
+constexpr int kWarps = 8;
+
+// Joins `n` partial results (max, sum at ml[2 i stride_ml], value at o[i * stride_o]) of one output value into (M, L, A)
+struct Joined {
+    float M, L, A;
+};
+__device__ __forceinline__ void join_part(Joined& j, float m, float l, float a) {
+    const float mn = fmaxf(j.M, m);
+    const float x = j.M == mn ? 1.0f : exp2_approx(j.M - mn), y = m == mn ? 1.0f : exp2_approx(m - mn);
+    j.L = fmaf(j.L, x, l * y);
+    j.A = fmaf(j.A, x, a * y);
+    j.M = mn;
+}
+
+// grid (batch * kv heads, query blocks, S) in clusters of S along z: the S CTAs of a cluster split the positions of one (sequence,
+// kv head); the warp that owns the last position appends the new token's row first.  Warps are joined through shared memory and
+// CTAs through distributed shared memory, head g by CTA g % S.
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kWarps * 32) attn_decode_int8_kernel(const DecodeArgs a) {
+    namespace cg = cooperative_groups;
+    using Attn = WarpAttention<HD, NQ>;
+    __shared__ __align__(16) uint8_t sm_q[NQ * Attn::kQueryBytes];
+    __shared__ float sm_unit[NQ];
+    __shared__ float sm_ml[kWarps][NQ][2];
+    __shared__ __align__(16) float sm_o[kWarps][NQ][HD];
+    __shared__ float sm_part_ml[NQ][2];
+    __shared__ __align__(16) float sm_part[NQ][HD];
     pdl_launch_dependents();
     pdl_wait();
-    const int b = blockIdx.x / n_kv, hk = blockIdx.x - b * n_kv, G = n_heads / n_kv;
+    const int b = blockIdx.x / a.n_kv, hk = blockIdx.x - b * a.n_kv, G = a.n_heads / a.n_kv;
+    const int q0 = blockIdx.y * NQ, nq = min(NQ, G - q0);             // this block's queries of the group
+    const int split = blockIdx.z, S = gridDim.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t pos = pos_p[b * pos_stride];
-    const bool live = pos >= 0 && pos < own.max_seq;
-    int64_t P = prefix_len ? *prefix_len : 0;
-    P = P < 0 ? 0 : (prefix_len && P > first.max_seq ? first.max_seq : P);
-    const float* row = qkv + b * qkv_stride + lane * VEC;
-    const int64_t base = (static_cast<int64_t>(b) * n_kv + hk) * own.max_seq;
-    float* orow = out + b * out_stride + static_cast<int64_t>(hk) * G * HD;
-    if (!live) {
-        for (int i = threadIdx.x; i < G * HD; i += kSimpleWarps * 32) orow[i] = 0.f;
-        return;
+    const int64_t pos = a.pos[b * a.pos_stride];
+    const bool live = pos >= 0 && pos < a.own.max_seq;
+    const int64_t P = prefix_rows(a);
+    const int n = live ? static_cast<int>(pos) + 1 : 0;
+    const int chunk = ((n + S - 1) / S + kTile - 1) / kTile * kTile;
+    const int t0 = min(static_cast<int64_t>(split) * chunk, static_cast<int64_t>(n)), t1 = min(static_cast<int64_t>(t0) + chunk, static_cast<int64_t>(n));
+    const int64_t base = (static_cast<int64_t>(b) * a.n_kv + hk) * a.own.max_seq;
+    const int8_t* kc = a.own.kc + base * HD;
+    const int8_t* vc = a.own.vc + base * HD;
+    const float* ks = a.own.ks + base;
+    const float* vs = a.own.vs + base;
+    const float* row = a.qkv + b * a.qkv_stride;
+    const float* cos_row = a.cos_t + (live ? P + pos : 0) * (HD / 2);
+    const float* sin_row = a.sin_t + (live ? P + pos : 0) * (HD / 2);
+
+    Attn w;
+    w.init(lane);
+    const int first = t0 + warp * kTile;
+    const bool owner = t1 == n && n > 0 && t1 > t0 && (n - 1 - t0) / kTile % kWarps == warp;
+    if (owner) {
+        // every query block of the group attends to the new row, so every one's owner writes it (the same bits)
+        float v[HD / 32];
+        load_row<HD>(v, row + static_cast<int64_t>(a.n_heads + hk) * HD, cos_row, sin_row, true, lane);
+        append_row<HD>(v, a.own.kc + (base + pos) * HD, a.own.ks + base + pos, lane);
+        load_row<HD>(v, row + static_cast<int64_t>(a.n_heads + a.n_kv + hk) * HD, cos_row, sin_row, false, lane);
+        append_row<HD>(v, a.own.vc + (base + pos) * HD, a.own.vs + base + pos, lane);
+        __syncwarp();
     }
-    auto rotated = [&](int64_t at, float (&v)[VEC], bool turn) {
+    if (first < t1) {
+        w.load_k(kc, ks, first, t1);
+        w.load_v(vc, vs, first, t1);
+    }
+    for (int q = warp; q < NQ; q += kWarps) {
+        float v[HD / 32];
+        if (q < nq && live) {
+            load_row<HD>(v, row + static_cast<int64_t>(hk * G + q0 + q) * HD, cos_row, sin_row, true, lane);
+        } else {
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) v[j] = row[at + j];
-        if (!turn) return;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
-            const float c = cos_t[(P + pos) * (HD / 2) + (lane & 15) * VEC + j], s = sin_t[(P + pos) * (HD / 2) + (lane & 15) * VEC + j];
-            float x1 = lane < 16 ? v[j] : other, x2 = lane < 16 ? other : v[j];
-            rotate_pair(x1, x2, c, s);
-            v[j] = lane < 16 ? x1 : x2;
+            for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
         }
-    };
-    if (warp < 2) {                       // warp 0 appends the key, warp 1 the value
-        float v[VEC];
-        rotated(static_cast<int64_t>(n_heads + (warp ? n_kv : 0) + hk) * HD, v, warp == 0);
-        float top = 1e-8f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) top = absmax_step(top, v[j]);
-        top = warp_max(top);
-        const float inv = __fdiv_rn(127.0f, top);
-        int8_t* codes = (warp ? own.vc : own.kc) + (base + pos) * HD + lane * VEC;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) codes[j] = static_cast<int8_t>(quantize_code<127, -127>(v[j], inv));
-        if (lane == 0) (warp ? own.vs : own.ks)[base + pos] = __fdiv_rn(top, 127.0f);
+        query_digits<HD>(v, sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
     }
     __syncthreads();
-    for (int g = 0; g < G; ++g) {
-        float q[VEC], acc[VEC];
-        rotated(static_cast<int64_t>(hk * G + g) * HD, q, true);
+    w.load_queries(sm_q, sm_unit);
+    w.run(kc, ks, vc, vs, first, t1, kWarps * kTile);
+    w.store(&sm_ml[warp][0][0], &sm_o[warp][0][0]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < nq * HD; i += kWarps * 32) {
+        const int q = i / HD, d = i % HD;
+        Joined j = {-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) { q[j] *= rsqrtf(static_cast<float>(HD)); acc[j] = 0.f; }
-        float m = -CUDART_INF_F, l = 0.f;
-        for (int64_t t = warp; t < P + pos + 1; t += kSimpleWarps) {
-            const CacheView& c = t < P ? first : own;
-            const int64_t at = t < P ? hk * first.max_seq + t : base + (t - P);
-            float d = 0.f;
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) d = fmaf(q[j], static_cast<float>(c.kc[at * HD + lane * VEC + j]), d);
-#pragma unroll
-            for (int o = 16; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
-            const float ksc = c.ks[at], vsc = c.vs[at];
-            const float s = fmaf(d, ksc, ksc - ksc);                 // NaN for a row whose scale is not finite
-            const float mn = fmaxf(m, s);
-            const float corr = m == -CUDART_INF_F ? 0.f : expf(m - mn);
-            const float p = s == -CUDART_INF_F ? 0.f : expf(s - mn);
-            l = fmaf(l, corr, p + (vsc - vsc));
-#pragma unroll
-            for (int j = 0; j < VEC; ++j) acc[j] = fmaf(acc[j], corr, p * vsc * static_cast<float>(c.vc[at * HD + lane * VEC + j]));
-            m = mn;
-        }
-        if (lane == 0) { sm_m[warp] = m; sm_l[warp] = l; }
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) sm_acc[warp][lane * VEC + j] = acc[j];
-        __syncthreads();
+        for (int u = 0; u < kWarps; ++u) join_part(j, sm_ml[u][q][0], sm_ml[u][q][1], sm_o[u][q][d]);
+        sm_part[q][d] = j.A;
+        if (d == 0) { sm_part_ml[q][0] = j.M; sm_part_ml[q][1] = j.L; }
+    }
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    const int64_t R = static_cast<int64_t>(a.batch) * G;
+    for (int q = split; q < nq; q += S) {
         if (threadIdx.x < HD) {
-            float M = -CUDART_INF_F, L = 0.f, A = 0.f;
-            for (int w = 0; w < kSimpleWarps; ++w) M = fmaxf(M, sm_m[w]);
-            for (int w = 0; w < kSimpleWarps; ++w) {
-                const float wgt = sm_m[w] == -CUDART_INF_F ? 0.f : expf(sm_m[w] - M);
-                L += sm_l[w] * wgt;
-                A += sm_acc[w][threadIdx.x] * wgt;
+            const int d = threadIdx.x;
+            Joined j = {-CUDART_INF_F, 0.f, 0.f};
+            for (int r = 0; r < S; ++r) {
+                const float* ml = cluster.map_shared_rank(&sm_part_ml[q][0], r);
+                join_part(j, ml[0], ml[1], cluster.map_shared_rank(&sm_part[q][0], r)[d]);
             }
-            orow[g * HD + threadIdx.x] = L == 0.f ? 0.f : A / L;
+            if (live) {
+                const int64_t at = (hk * R + static_cast<int64_t>(b) * G + q0 + q) * a.parts;
+                for (int p = 0; p < a.parts; ++p) join_part(j, a.part_ml[2 * (at + p)], a.part_ml[2 * (at + p) + 1], a.part_o[(at + p) * HD + d]);
+            }
+            const float o = j.L == 0.f ? 0.f : j.A / j.L;
+            a.out[b * a.out_stride + static_cast<int64_t>(hk * G + q0 + q) * HD + d] = o;
+            sm_o[0][0][d] = o;
         }
-        __syncthreads();
+        if (a.planes != nullptr) {
+            // the same values as prepared activations of the [batch, n_heads * HD] matrix: a head is HD / 32 whole groups
+            __syncthreads();
+            if (warp == 0) {
+                const bool in = lane < HD / 8;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = in ? sm_o[0][0][lane * 8 + j] : 0.f;
+                const PreparedParts pp = prepared_parts(a.planes, static_cast<size_t>(a.n_heads) * (HD / 32), a.nmain, a.nlow);
+                convert_groups<kOrderNibble>(v, b, a.batch, static_cast<size_t>(hk * G + q0 + q) * (HD / 32), a.pmode, a.nmain, a.nlow, 0.0625f, pp, in);
+            }
+            __syncthreads();
+        }
+    }
+    cluster.sync();                                                    // keeps shared memory alive until it has been read
+}
+
+// Partial attention of every sequence's queries to the shared prefix.  grid (kv heads, splits of the prefix, blocks of 8 QW rows),
+// the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; QW warps of a block take
+// the same positions (their loads meet in L1) and the KW = 8 / QW groups of warps take alternate tiles.
+template <int HD>
+__global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const DecodeArgs a, int QW, float* __restrict__ part_ml, float* __restrict__ part_o) {
+    constexpr int NQ = 8;
+    using Attn = WarpAttention<HD, NQ>;
+    constexpr int kDigits = kWarps * NQ * Attn::kQueryBytes, kOuts = kWarps * NQ * HD * 4;
+    __shared__ __align__(16) uint8_t sm[kDigits > kOuts ? kDigits : kOuts];      // the queries' digits, then the warps' outputs
+    __shared__ float sm_unit[kWarps * NQ];
+    __shared__ float sm_ml[kWarps][NQ][2];
+    pdl_launch_dependents();
+    pdl_wait();
+    const int hk = blockIdx.x, split = blockIdx.y, splits = gridDim.y, G = a.n_heads / a.n_kv;
+    const int64_t R = static_cast<int64_t>(a.batch) * G, r0 = static_cast<int64_t>(blockIdx.z) * QW * NQ;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, KW = kWarps / QW, qg = warp % QW, kw = warp / QW;
+    const int n = static_cast<int>(prefix_rows(a));
+    const int chunk = ((n + splits - 1) / splits + kTile - 1) / kTile * kTile;
+    const int t0 = min(static_cast<int64_t>(split) * chunk, static_cast<int64_t>(n)), t1 = min(static_cast<int64_t>(t0) + chunk, static_cast<int64_t>(n));
+    const int64_t base = static_cast<int64_t>(hk) * a.first.max_seq;
+    const int8_t* kc = a.first.kc + base * HD;
+    const int8_t* vc = a.first.vc + base * HD;
+    const float* ks = a.first.ks + base;
+    const float* vs = a.first.vs + base;
+    Attn w;
+    w.init(lane);
+    const int first = t0 + kw * kTile;
+    if (first < t1) {
+        w.load_k(kc, ks, first, t1);
+        w.load_v(vc, vs, first, t1);
+    }
+    for (int i = warp; i < QW * NQ; i += kWarps) {
+        const int64_t r = r0 + i;
+        const int64_t b = r < R ? r / G : 0;
+        const int64_t pos = a.pos[b * a.pos_stride];
+        float v[HD / 32];
+        if (r < R && pos >= 0 && pos < a.own.max_seq) {
+            load_row<HD>(v, a.qkv + b * a.qkv_stride + (hk * G + r - b * G) * HD, a.cos_t + (n + pos) * (HD / 2), a.sin_t + (n + pos) * (HD / 2), true, lane);
+        } else {
+#pragma unroll
+            for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
+        }
+        query_digits<HD>(v, sm + i * Attn::kQueryBytes, sm_unit + i, lane);
+    }
+    __syncthreads();
+    w.load_queries(sm + qg * NQ * Attn::kQueryBytes, sm_unit + qg * NQ);
+    w.run(kc, ks, vc, vs, first, t1, KW * kTile);
+    __syncthreads();                                                    // everyone has read the digits
+    float* sm_o = reinterpret_cast<float*>(sm);
+    w.store(&sm_ml[warp][0][0], sm_o + warp * NQ * HD);
+    __syncthreads();
+    for (int i = threadIdx.x; i < QW * NQ * HD; i += kWarps * 32) {
+        const int q = i / HD, d = i % HD;
+        if (r0 + q >= R) break;
+        Joined j = {-CUDART_INF_F, 0.f, 0.f};
+        for (int u = 0; u < KW; ++u) {
+            const int wi = q / NQ + u * QW;
+            join_part(j, sm_ml[wi][q % NQ][0], sm_ml[wi][q % NQ][1], sm_o[(wi * NQ + q % NQ) * HD + d]);
+        }
+        const int64_t at = (hk * R + r0 + q) * splits + split;
+        part_o[at * HD + d] = j.A;
+        if (d == 0) { part_ml[2 * at] = j.M; part_ml[2 * at + 1] = j.L; }
     }
 }
 
@@ -244,12 +672,61 @@ int check_cache_pointers(const sgqd_cache_int8* c) {
 }
 CacheView view(const sgqd_cache_int8* c) { return CacheView{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->max_seq}; }
 
+// Splits of a shared prefix and rows per block of its kernel: a function of the sizes alone, so that the workspace's size is one
+// too.  148 SMs, one block each.
+constexpr int kPrefixBlocks = 148;
+struct PrefixPlan {
+    int qw, blocks, splits;
+    int64_t rows;                        // (kv head, query row) pairs
+    size_t off_o, bytes;
+};
+PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t prefix_max) {
+    PrefixPlan p = {};
+    const int64_t R = batch * (n_heads / n_kv);
+    p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : (R <= 32 ? 4 : 8));
+    p.blocks = static_cast<int>(ceil_div(R, 8 * p.qw));
+    const int64_t most = ceil_div(prefix_max, kTile * (kWarps / p.qw));              // a tile for every warp
+    int64_t s = kPrefixBlocks / (n_kv * p.blocks);
+    s = s < 1 ? 1 : (s > most ? most : s);
+    p.splits = static_cast<int>(s > 65535 ? 65535 : s);
+    p.rows = n_kv * R;
+    p.off_o = (static_cast<size_t>(p.rows) * p.splits * 8 + 255) / 256 * 256;
+    p.bytes = p.off_o + static_cast<size_t>(p.rows) * p.splits * head_dim * 4;
+    return p;
+}
+
+template <int HD, int NQ>
+int launch_decode(const DecodeArgs& a, int64_t batch, cudaStream_t s) {
+    const int G = a.n_heads / a.n_kv, blocks = (G + NQ - 1) / NQ;
+    const int64_t units = batch * a.n_kv * blocks;
+    // splits of the positions: a block per SM slot, at least a tile for each of its warps, at most the portable cluster size
+    int64_t S = 2 * static_cast<int64_t>(sm_count()) / units;
+    const int64_t most = ceil_div(a.own.max_seq, kTile * kWarps);
+    S = S > most ? most : S;
+    S = S > 8 ? 8 : (S < 1 ? 1 : S);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(static_cast<unsigned>(batch * a.n_kv), static_cast<unsigned>(blocks), static_cast<unsigned>(S));
+    cfg.blockDim = dim3(kWarps * 32);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = static_cast<unsigned>(S);
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    SGQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_decode_int8_kernel<HD, NQ>, a));
+    return SGQ_OK;
+}
+
 int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table, int64_t table_rows,
-                const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix, const int32_t* prefix_len, float* out,
-                int64_t out_stride, void* prepared_out, size_t prepared_bytes, cudaStream_t s) {
+                const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix, const int32_t* prefix_len,
+                float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes, void* workspace, size_t workspace_bytes, cudaStream_t s) {
     int rc = check_cache(cache);
     if (rc != SGQ_OK) return rc;
-    const int64_t hd = cache->head_dim, kv = cache->n_kv_heads;
+    const int64_t hd = cache->head_dim, kv = cache->n_kv_heads, batch = cache->batch;
     if (hd != 64 && hd != 128) return bad(SGQ_ERR_UNSUPPORTED, "head_dim must be 64 or 128");
     if (n_heads <= 0 || n_heads > 65535 || n_heads % kv) return bad(SGQ_ERR_BAD_SHAPE, "n_heads must be a multiple of the cache's heads");
     if (qkv_stride < (n_heads + 2 * kv) * hd || out_stride < n_heads * hd) return bad(SGQ_ERR_BAD_SHAPE, "row stride too small");
@@ -259,25 +736,42 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
         if (prefix->batch != 1 || prefix->n_kv_heads != kv || prefix->head_dim != hd)
             return bad(SGQ_ERR_BAD_SHAPE, "the prefix is one sequence with the cache's heads");
     }
+    if (cache->max_seq > kMaxPositions || (prefix && prefix->max_seq > kMaxPositions)) return bad(SGQ_ERR_BAD_SHAPE, "more than 2^30 positions");
     if (table_rows < cache->max_seq + (prefix ? prefix->max_seq : 0)) return bad(SGQ_ERR_BAD_SHAPE, "the cos / sin tables are too short");
-    if (cache->batch == 0) return SGQ_OK;
+    if (batch == 0) return SGQ_OK;
     if (!qkv || !cos_table || !sin_table || !pos || !out || (prefix && !prefix_len)) return bad(SGQ_ERR_NULL_POINTER, "NULL argument");
     if ((rc = check_cache_pointers(cache)) != SGQ_OK || (prefix && (rc = check_cache_pointers(prefix)) != SGQ_OK)) return rc;
     if (!aligned(qkv, 16) || (qkv_stride & 3) || !aligned(cos_table, 16) || !aligned(sin_table, 16))
         return bad(SGQ_ERR_ALIGNMENT, "qkv rows and tables must be 16-byte aligned");
     PreparedLayout L = {};
-    if ((rc = check_prepared(prepared_out, prepared_bytes, cache->batch, n_heads * hd, &L)) != SGQ_OK) return rc;
+    if ((rc = check_prepared(prepared_out, prepared_bytes, batch, n_heads * hd, &L)) != SGQ_OK) return rc;
+    PrefixPlan plan = {};
+    if (prefix) {
+        plan = prefix_plan(batch, n_heads, kv, hd, prefix->max_seq);
+        if (plan.blocks > 65535) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
+        if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 256)) return bad(SGQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
+    }
     if ((rc = check_device()) != SGQ_OK) return rc;
-    const CacheView own = view(cache), first = prefix ? view(prefix) : CacheView{};
-    const dim3 grid(static_cast<unsigned>(cache->batch * kv));
-    if (hd == 128)
-        SGQ_CUDA_TRY(launch_kernel(attn_decode_int8_kernel<128>, grid, dim3(kSimpleWarps * 32), 0, s, true, qkv, qkv_stride, static_cast<int>(n_heads),
-                                   static_cast<int>(kv), cos_table, sin_table, pos, pos_stride, own, first, prefix_len, out, out_stride));
-    else
-        SGQ_CUDA_TRY(launch_kernel(attn_decode_int8_kernel<64>, grid, dim3(kSimpleWarps * 32), 0, s, true, qkv, qkv_stride, static_cast<int>(n_heads),
-                                   static_cast<int>(kv), cos_table, sin_table, pos, pos_stride, own, first, prefix_len, out, out_stride));
-    if (prepared_out) return sgq_prepare_x(out, cache->batch, n_heads * hd, prepared_out, prepared_bytes, s);
-    return SGQ_OK;
+    DecodeArgs a = {};
+    a.qkv = qkv; a.qkv_stride = qkv_stride; a.n_heads = static_cast<int>(n_heads); a.n_kv = static_cast<int>(kv); a.batch = static_cast<int>(batch);
+    a.cos_t = cos_table; a.sin_t = sin_table; a.pos = pos; a.pos_stride = pos_stride; a.own = view(cache);
+    a.out = out; a.out_stride = out_stride; a.pmode = L.mode; a.nmain = L.nmain; a.nlow = L.nlow; a.planes = static_cast<uint8_t*>(prepared_out);
+    if (prefix) {
+        a.first = view(prefix);
+        a.prefix_len = prefix_len;
+        float* ml = static_cast<float*>(workspace);
+        float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.off_o);
+        const dim3 grid(static_cast<unsigned>(kv), static_cast<unsigned>(plan.splits), static_cast<unsigned>(plan.blocks));
+        if (hd == 128) SGQ_CUDA_TRY(launch_kernel(attn_prefix_int8_kernel<128>, grid, dim3(kWarps * 32), 0, s, true, a, plan.qw, ml, o));
+        else SGQ_CUDA_TRY(launch_kernel(attn_prefix_int8_kernel<64>, grid, dim3(kWarps * 32), 0, s, true, a, plan.qw, ml, o));
+        a.part_ml = ml;
+        a.part_o = o;
+        a.parts = plan.splits;
+    }
+    // four queries per warp where the group has no more: 2 column sets in the place of 3 and half the outputs in registers
+    const bool four = n_heads / kv <= 4;
+    if (hd == 128) return four ? launch_decode<128, 4>(a, batch, s) : launch_decode<128, 8>(a, batch, s);
+    return four ? launch_decode<64, 4>(a, batch, s) : launch_decode<64, 8>(a, batch, s);
 }
 
 }  // namespace
@@ -348,22 +842,23 @@ int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads,
                           int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, float* out, int64_t out_stride,
                           void* prepared_out, size_t prepared_bytes, void* stream) {
     return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, nullptr, nullptr, out, out_stride, prepared_out,
-                       prepared_bytes, static_cast<cudaStream_t>(stream));
+                       prepared_bytes, nullptr, 0, static_cast<cudaStream_t>(stream));
 }
 
 size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t prefix_max) {
-    (void)batch; (void)n_heads; (void)n_kv_heads; (void)head_dim; (void)prefix_max;
-    return 0;
+    if (batch <= 0 || batch > 0x7fffffff || n_heads <= 0 || n_heads > 65535 || n_kv_heads <= 0 || n_heads % n_kv_heads || prefix_max <= 0 ||
+        prefix_max > kMaxPositions || (head_dim != 64 && head_dim != 128))
+        return 0;
+    return prefix_plan(batch, n_heads, n_kv_heads, head_dim, prefix_max).bytes;
 }
 
 int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table,
                                  int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix,
                                  const int32_t* prefix_len, float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes,
                                  void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace; (void)workspace_bytes;
     if (!prefix) return bad(SGQ_ERR_NULL_POINTER, "prefix is NULL");
     return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, prefix, prefix_len, out, out_stride, prepared_out,
-                       prepared_bytes, static_cast<cudaStream_t>(stream));
+                       prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"
