@@ -160,19 +160,23 @@ SGQ_API int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_
  * read.  The query and the softmax weights enter exact integer products as 24-bit fixed point (the query relative to its
  * largest value, the weights relative to the largest of every 32 positions), sums are fp32: errors are those of an fp32
  * evaluation.  table_rows >= max_seq.  head_dim must be 64 or 128, max_seq at most
- * 2^30.  prepared_out: as for sgqd_attn_decode. */
+ * 2^30.  prepared_out: as for sgqd_attn_decode.  workspace: as many bytes as the query says (0: none is read; caches that
+ * may grow long need some), 256-byte aligned; it holds nothing from one call to the next, and calls that may run at the
+ * same time need one each.  The query's answer follows from the sizes alone. */
+SGQ_API size_t sgqd_attn_decode_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                                                     int64_t max_seq);
 SGQ_API int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,
                                   const float* sin_table, int64_t table_rows, const int32_t* pos, int64_t pos_stride,
-                                  const sgqd_cache_int8* cache, float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes, void* stream);
+                                  const sgqd_cache_int8* cache, float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes, void* workspace, size_t workspace_bytes,
+                                  void* stream);
 
 /* The same for sequences that begin with the same *prefix_len tokens (ONE DEVICE int32, taken as at least 0 and at most
  * prefix->max_seq), whose rows lie once in `prefix`, a cache of one sequence with the same heads: every query attends to
  * the prefix rows and to its own rows 0 .. pos[b], which stand at positions *prefix_len + t of its sequence (the rotation of
  * the new token included; table_rows >= prefix->max_seq + max_seq).  The prefix is read once for the whole
- * batch.  workspace: as many bytes as the query says (0 for sizes that are refused), 256-byte aligned; it holds nothing from one call to the
- * next, and calls that may run at the same time need one each. */
+ * batch.  workspace: as for sgqd_attn_decode_int8 (0 bytes only for sizes that are refused). */
 SGQ_API size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
-                                                            int64_t prefix_max);
+                                                            int64_t max_seq, int64_t prefix_max);
 SGQ_API int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,
                                          const float* sin_table, int64_t table_rows, const int32_t* pos,
                                          int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix, const int32_t* prefix_len,

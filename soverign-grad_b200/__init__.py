@@ -46,7 +46,7 @@ EXPORTS = [
 DECODER_EXPORTS = ["sgqd_add_rmsnorm", "sgqd_rope_kv_store", "sgqd_attn_decode", "sgqd_silu_mul", "sgqd_embedding",
                    "sgqd_argmax_rows", "sgqd_attn_prefill", "sgqd_attn_prefill_bf16", "sgqd_attn_decode_allgather",
                    "sgqd_silu_mul_allgather", "sgqd_rope_kv_store_int8", "sgqd_kv_load_int8", "sgqd_attn_decode_int8",
-                   "sgqd_attn_decode_prefix_int8", "sgqd_attn_decode_prefix_int8_workspace_bytes"]
+                   "sgqd_attn_decode_prefix_int8", "sgqd_attn_decode_prefix_int8_workspace_bytes", "sgqd_attn_decode_int8_workspace_bytes"]
 
 
 class SgqError(RuntimeError):
@@ -116,10 +116,12 @@ def _load() -> C.CDLL:
     cache = C.POINTER(CacheInt8)
     lib.sgqd_rope_kv_store_int8.argtypes = [p, i64, i64, i64, p, p, i64, p, i64, p, p, p, i64, cache, p]
     lib.sgqd_kv_load_int8.argtypes = [cache, i64, i64, p, p, i64, i64, p]
-    lib.sgqd_attn_decode_int8.argtypes = [p, i64, i64, p, p, i64, p, i64, cache, p, i64, p, sz, p]
+    lib.sgqd_attn_decode_int8.argtypes = [p, i64, i64, p, p, i64, p, i64, cache, p, i64, p, sz, p, sz, p]
     lib.sgqd_attn_decode_prefix_int8.argtypes = [p, i64, i64, p, p, i64, p, i64, cache, cache, p, p, i64, p, sz, p, sz, p]
     lib.sgqd_attn_decode_prefix_int8_workspace_bytes.restype = sz
-    lib.sgqd_attn_decode_prefix_int8_workspace_bytes.argtypes = [i64, i64, i64, i64, i64]
+    lib.sgqd_attn_decode_prefix_int8_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, i64]
+    lib.sgqd_attn_decode_int8_workspace_bytes.restype = sz
+    lib.sgqd_attn_decode_int8_workspace_bytes.argtypes = [i64, i64, i64, i64, i64]
     return lib
 
 
@@ -356,11 +358,12 @@ def kv_load_int8(cache: KVCacheInt8, rows: int, *, batch: Optional[int] = None, 
 
 
 def attn_decode_int8(qkv: torch.Tensor, cache: KVCacheInt8, cos: torch.Tensor, sin: torch.Tensor, pos: torch.Tensor, n_heads: int, *,
-                     out: Optional[torch.Tensor] = None, prepared: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     out: Optional[torch.Tensor] = None, prepared: Optional[torch.Tensor] = None,
+                     workspace: Optional[Workspace] = None) -> torch.Tensor:
     """One new token per sequence (qkv[batch, width], position pos[b]): appends it to the cache as rope_kv_store_int8 does and
     returns its attention to positions 0 .. pos[b], [batch, n_heads * head_dim].  A sequence with pos outside the cache
     takes no part (zeros).  prepared: also writes the output's prepared form (prepared_x_bytes), for linear_int4_prepared."""
-    return _native.attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared)
+    return _native.attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared, workspace)
 
 
 def attn_decode_prefix_int8(qkv: torch.Tensor, cache: KVCacheInt8, prefix: KVCacheInt8, prefix_len: torch.Tensor, cos: torch.Tensor,

@@ -11,6 +11,7 @@
 
 #include "../../include/sgq_decoder.h"
 
+#include <algorithm>
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -131,17 +132,17 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t
 // base-256 digits (the arithmetic of gemv_prepare.cuh), one digit per column of the small operand.
 //
 //   scores   A = 16 rows of the cache x 32 values, B = 32 values x 8 columns.  A lane (g, t) = (lane / 4, lane % 4) of the
-//            warp loads the 16-byte chunks t (and 4 + t) of the rows 4g .. 4g+3 of a tile of 32 positions: these ARE the A
+//            warp reads the 16-byte chunks t (and 4 + t) of the rows 4g .. 4g+3 of a tile of 32 positions: these ARE the A
 //            fragments, the order of the head dimension inside them being the same in the query's digits.  Columns 2t, 2t+1
 //            of a "main" column set hold digits 2 and 1 of query t, those of the "low" set digit 0 of queries t and
 //            t + 4, so a lane finds all digits of its one or two queries in its own accumulators.
 //   weights  w = p * value scale, relative to the largest |w| of the tile and query: their digits cross the warp by shuffles
 //            (rows of the accumulators become the contraction index).
-//   output   A = 16 values x 32 positions: a lane loads HD/8 consecutive values of 8 positions and transposes 4 x 4 bytes
+//   output   A = 16 values x 32 positions: a lane reads HD/8 consecutive values of 8 positions and transposes 4 x 4 bytes
 //            with byte permutes.  B = 32 positions x 8 columns of weight digits.
 //
-// Scores and outputs leave the integer domain once per tile (sum of 32 or HD products below 2^22, exact as fp32), scaled
-// and added in fp32 with the running maximum and sum of the softmax.  A lane holds the scores of positions 4g .. 4g+3 and
+// Scores and outputs leave the integer domain once per tile or step (sums of at most 128 products, below 2^21.1), scaled
+// and added in fp32 with the running reference and sum of the softmax.  A lane holds the scores of positions 4g .. 4g+3 and
 // the values [HD/8 g, HD/8 (g+1)) of the outputs of queries t and t + 4.
 struct CacheView {
     int8_t* kc;
@@ -151,21 +152,20 @@ struct CacheView {
     int64_t max_seq;
 };
 
-// D = A(16x32, s8) * B(32x8, s8) + magic (see gemv_prepare.cuh: the sum read as fp32 bits is 12582912 + S), and D += A * B
+// D = A(16x32, s8) * B(32x8, s8), and D += A * B
 __device__ __forceinline__ void mma_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
         : "=r"(d[0]), "=r"(d[1]), "=r"(d[2]), "=r"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(kMagicBits));
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
 }
 __device__ __forceinline__ void mma_next(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// digit sums (2: highest) of one exact sum, as fp32
+// The exact sum whose digit sums (2: highest; each below 2^21.1) these are, as fp32.  256 d2 + d1 fits an int32.
 __device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
-    const float f2 = __int_as_float(d2) - kMagicF, f1 = __int_as_float(d1) - kMagicF, f0 = __int_as_float(d0) - kMagicF;
-    return fmaf(f2, 65536.0f, fmaf(f1, 256.0f, f0));
+    return fmaf(static_cast<float>(d2 * 256 + d1), 256.0f, static_cast<float>(d0));
 }
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
@@ -180,17 +180,77 @@ __device__ __forceinline__ float exp2_approx(float x) {
 
 constexpr int kTile = 32;              // positions per step of a warp
 
-// One warp's running attention of up to NQ (4 or 8) queries over tiles of one kv head's rows.
-template <int HD, int NQ>
+// ---- half tiles in shared memory: the 32 rows of keys or of values and their scales, fetched by cp.async -------------------
+// Rows lie in 128-byte lines of eight 16-byte chunks whose place is permuted by the row, so that the fragment reads (for keys
+// the chunks t of rows 4g + i, for values the chunk g of rows 4t + i) touch all banks.
+template <int HD>
+struct Half {
+    static constexpr int kScales = kTile * HD, kBytes = kScales + kTile * 4;
+    static __device__ __forceinline__ int place(int row, int chunk, int turn) {
+        if constexpr (HD == 128) return row * 128 + ((chunk ^ turn) << 4);
+        else return (row >> 1) * 128 + ((((row & 1) * 4 + chunk) ^ turn) << 4);
+    }
+    static __device__ __forceinline__ int key_at(int row, int chunk) { return place(row, chunk, ((row >> 2) & 1) * 4); }
+    static __device__ __forceinline__ int value_at(int row, int chunk) { return place(row, chunk, ((row >> 2) & 3) * 2); }
+    template <bool KEYS>
+    static __device__ __forceinline__ int at(int row, int chunk) { return KEYS ? key_at(row, chunk) : value_at(row, chunk); }
+};
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// `THREADS` threads (this one is number i) ask for the rows codes[t ..] and their scales; rows from t1 on repeat the last one
+// (their positions are masked).
+template <int HD, int THREADS, bool KEYS>
+__device__ __forceinline__ void request_half(uint32_t dst, const int8_t* codes, const float* scales, int t, int t1, int i) {
+    constexpr int CH = HD / 16, USED = THREADS < kTile * CH ? THREADS : kTile * CH, STEP = USED / CH;
+    const int last = t1 - 1 - t, row0 = i / CH, c = i % CH;
+    if (USED == THREADS || i < USED) {
+        const int8_t* from = codes + static_cast<int64_t>(t) * HD + c * 16;
+        // where the row's chunk goes differs from row to row by a multiple of the line and by which bits of the place are flipped
+        uint32_t to[kTile / STEP];
+#pragma unroll
+        for (int x = 0; x < kTile / STEP; ++x) to[x] = dst + Half<HD>::template at<KEYS>(row0 + x * STEP, c);
+        if (last >= kTile - 1) {
+            from += row0 * HD;
+#pragma unroll
+            for (int x = 0; x < kTile / STEP; ++x) cp_async_16(to[x], from + x * STEP * HD);
+        } else {
+#pragma unroll
+            for (int x = 0; x < kTile / STEP; ++x) cp_async_16(to[x], from + min(row0 + x * STEP, last) * HD);
+        }
+    }
+    if (THREADS == 32 || i < 32) cp_async_4(dst + Half<HD>::kScales + 4 * (i & 31), scales + t + min(i & 31, last));
+}
+// A group: ST half tiles `step` positions apart, the first one at position t
+template <int HD, int THREADS, int ST, bool KEYS>
+__device__ __forceinline__ void request_group(uint32_t dst, const int8_t* codes, const float* scales, int t, int step, int t1, int i) {
+#pragma unroll
+    for (int j = 0; j < ST; ++j)
+        if (t + j * step < t1) request_half<HD, THREADS, KEYS>(dst + j * Half<HD>::kBytes, codes, scales, t + j * step, t1, i);
+}
+// A warp's ring holds three groups: keys, values, keys of the next step, values of the next step, ... in turn.  While one of them
+// is in use the two behind it are on their way.
+constexpr int kGroups = 3;
+__device__ __forceinline__ int next_slot(int s) { return s + 1 == kGroups ? 0 : s + 1; }
+
+// One warp's running attention of up to NQ (4 or 8) queries over tiles of one kv head's rows, ST tiles per step.
+template <int HD, int NQ, int ST>
 struct WarpAttention {
     static constexpr int KW = HD / 16;         // 32-bit words of a key row per lane
     static constexpr int VB = HD / 8;          // values per lane and position
     static constexpr int VW = VB / 4;
     static constexpr int NS = NQ / 4, NT = NS + 1;
     static constexpr int kQueryBytes = 3 * HD; // digit planes of one query: [digit][HD]
+    static constexpr float kAhead = 6.0f;
 
-    uint32_t k[4][KW], v[8][VW], bq[NT][KW];
-    float ks[4], vs[4];
+    uint32_t bq[NT][KW];
     float qu[NS], m[NS], l[NS], o[NS][VB];
     int g, t;
 
@@ -223,52 +283,27 @@ struct WarpAttention {
         if (NS == 2) rd(bq[NS], (g >> 1) + 4 * (g & 1), 0, false);
         else rd(bq[NS], g >> 1, 0, (g & 1) != 0);
     }
-    __device__ __forceinline__ void load_k(const int8_t* kc, const float* ksc, int t0, int t1) {
+    // scores of a tile's keys: sc[s][i] of position 4g + i and query t + 4s, in base-2 units; positions from `n` on are masked
+    __device__ __forceinline__ void scores(float (&sc)[NS][4], const uint8_t* tile, int n) {
+        uint32_t k[4][KW];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int key = t0 + 4 * g + i;
-            key = key < t1 ? key : t1 - 1;                    // clamped: masked in step()
-            const uint4* p = reinterpret_cast<const uint4*>(kc + static_cast<int64_t>(key) * HD + 16 * t);
+        for (int i = 0; i < 4; ++i)
 #pragma unroll
             for (int c = 0; c < KW / 4; ++c) {
-                const uint4 x = p[4 * c];
+                const uint4 x = *reinterpret_cast<const uint4*>(tile + Half<HD>::key_at(4 * g + i, t + 4 * c));
                 k[i][4 * c] = x.x; k[i][4 * c + 1] = x.y; k[i][4 * c + 2] = x.z; k[i][4 * c + 3] = x.w;
             }
-            ks[i] = ksc[key];
-        }
-    }
-    __device__ __forceinline__ void load_v(const int8_t* vc, const float* vsc, int t0, int t1) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            int key = t0 + 4 * g + i;
-            key = key < t1 ? key : t1 - 1;
-            vs[i] = vsc[key];
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            int key = t0 + 4 * t + (i & 3) + 16 * (i >> 2);
-            key = key < t1 ? key : t1 - 1;
-            const int8_t* p = vc + static_cast<int64_t>(key) * HD + VB * g;
-            if constexpr (VW == 4) {
-                const uint4 x = *reinterpret_cast<const uint4*>(p);
-                v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
-            } else {
-                const uint2 x = *reinterpret_cast<const uint2*>(p);
-                v[i][0] = x.x; v[i][1] = x.y;
-            }
-        }
-    }
-    // scores of the loaded keys: sc[s][i] of position t0 + 4g + i and query t + 4s, in base-2 units
-    __device__ __forceinline__ void scores(float (&sc)[NS][4], int t0, int t1) {
+        const float4 ks4 = *reinterpret_cast<const float4*>(tile + Half<HD>::kScales + 16 * g);
+        const float ks[4] = {ks4.x, ks4.y, ks4.z, ks4.w};
         int acc[2][NT][4];
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                mma_first(acc[h][n], k[2 * h][0], k[2 * h + 1][0], k[2 * h][1], k[2 * h + 1][1], bq[n][0], bq[n][1]);
+            for (int n2 = 0; n2 < NT; ++n2) {
+                mma_first(acc[h][n2], k[2 * h][0], k[2 * h + 1][0], k[2 * h][1], k[2 * h + 1][1], bq[n2][0], bq[n2][1]);
 #pragma unroll
                 for (int c = 1; c < KW / 2; ++c)
-                    mma_next(acc[h][n], k[2 * h][2 * c], k[2 * h + 1][2 * c], k[2 * h][2 * c + 1], k[2 * h + 1][2 * c + 1], bq[n][2 * c], bq[n][2 * c + 1]);
+                    mma_next(acc[h][n2], k[2 * h][2 * c], k[2 * h + 1][2 * c], k[2 * h][2 * c + 1], k[2 * h + 1][2 * c + 1], bq[n2][2 * c], bq[n2][2 * c + 1]);
             }
 #pragma unroll
         for (int s = 0; s < NS; ++s)
@@ -276,119 +311,167 @@ struct WarpAttention {
             for (int i = 0; i < 4; ++i) {
                 const int h = i >> 1, r = 2 * (i & 1);
                 const float x = join_digits(acc[h][s][r], acc[h][s][r + 1], acc[h][NS][r + s]) * qu[s];
-                const float y = fmaf(x, ks[i], ks[i] - ks[i]);          // NaN for a row whose scale is not finite
-                sc[s][i] = t0 + 4 * g + i < t1 ? y : -CUDART_INF_F;
+                sc[s][i] = fmaf(x, ks[i], ks[i] - ks[i]);               // NaN for a row whose scale is not finite
             }
+        if (n < kTile) {
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    if (4 * g + i >= n) sc[s][i] = -CUDART_INF_F;
+        }
     }
-    // the tile's weights into the running softmax, and its values into the outputs
-    __device__ __forceinline__ void accumulate(float (&sc)[NS][4], int t0, int t1) {
-        uint32_t bw[NT][2];
-        float corr[NS], unit[NS];
-        uint32_t w0[NS], w1[NS], w2[NS];
+    __device__ __forceinline__ void scores_of(float (&sc)[ST][NS][4], const uint8_t* keys, const int (&n)[ST]) {
+#pragma unroll
+        for (int j = 0; j < ST; ++j) scores(sc[j], keys + j * Half<HD>::kBytes, n[j]);
+    }
+    // A group of values, of which tile j has n[j] positions, with the scores: into the running sums and the outputs.  The
+    // weights are taken against a reference that follows the maximum only when a score exceeds it by kAhead (weights up to
+    // 2^kAhead): most steps then neither wait for a maximum to cross the warp nor rescale anything.
+    __device__ __forceinline__ void accumulate(float (&sc)[ST][NS][4], const uint8_t* values, const int (&n)[ST]) {
+        uint32_t bw[ST][NT][2];
+        float unit[NS];
+        uint32_t w0[ST][NS], w1[ST][NS], w2[ST][NS];
+        float top[NS];
+        bool ahead = false;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            float top = fmaxf(fmaxf(sc[s][0], sc[s][1]), fmaxf(sc[s][2], sc[s][3]));
+            top[s] = -CUDART_INF_F;
 #pragma unroll
-            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-            const float mn = fmaxf(m[s], top);
-            corr[s] = m[s] == mn ? 1.0f : exp2_approx(m[s] - mn);
-            m[s] = mn;
-            float w[4], sum = 0.f, most = 0.f;
+            for (int j = 0; j < ST; ++j) top[s] = fmaxf(top[s], fmaxf(fmaxf(sc[j][s][0], sc[j][s][1]), fmaxf(sc[j][s][2], sc[j][s][3])));
+            ahead |= top[s] > m[s] + kAhead;
+        }
+        if (__any_sync(0xffffffffu, ahead)) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float p = sc[s][i] == -CUDART_INF_F ? 0.f : exp2_approx(sc[s][i] - mn);
-                sum += p;
-                w[i] = p * (t0 + 4 * g + i < t1 ? vs[i] : 0.f);
-                most = max_nan(most, fabsf(w[i]));
+            for (int s = 0; s < NS; ++s) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) top[s] = fmaxf(top[s], __shfl_xor_sync(0xffffffffu, top[s], d));
+                const float mn = fmaxf(m[s], top[s]), corr = m[s] == mn ? 1.0f : exp2_approx(m[s] - mn);
+                m[s] = mn;
+                l[s] *= corr;
+#pragma unroll
+                for (int j = 0; j < VB; ++j) o[s][j] *= corr;
             }
-            l[s] = fmaf(l[s], corr[s], sum);
+        }
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            float most = 0.f;
+            const float ref = m[s] == -CUDART_INF_F ? 0.f : m[s];        // nothing but masked positions so far: weights of zero
+#pragma unroll
+            for (int j = 0; j < ST; ++j) {
+                const float4 v4 = *reinterpret_cast<const float4*>(values + j * Half<HD>::kBytes + Half<HD>::kScales + 16 * g);
+                float vs[4] = {v4.x, v4.y, v4.z, v4.w};
+                if (n[j] < kTile) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (4 * g + i >= n[j]) vs[i] = 0.f;               // whatever a masked position's scale is
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float p = exp2_approx(sc[j][s][i] - ref);
+                    l[s] += p;
+                    sc[j][s][i] = p * vs[i];
+                    most = max_nan(most, fabsf(sc[j][s][i]));
+                }
+            }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-            // a tile whose weights vanish against the running maximum contributes nothing; NaN and infinity pass
+            // weights that vanish against the reference contribute nothing; NaN and infinity pass
             const float per = most < 1e-30f ? 0.f : __fdividef(kDigitRange, most);
             unit[s] = most * (1.0f / kDigitRange);
-            uint32_t d[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) d[i] = digit_bytes(__float2int_rn(w[i] * per));
-            const uint32_t x = __byte_perm(d[0], d[1], 0x5140), y = __byte_perm(d[2], d[3], 0x5140);
-            w0[s] = __byte_perm(x, y, 0x5410);
-            w1[s] = __byte_perm(x, y, 0x7632);
-            w2[s] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+            for (int j = 0; j < ST; ++j) {
+                uint32_t d[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) d[i] = digit_bytes(__float2int_rn(sc[j][s][i] * per));
+                const uint32_t x = __byte_perm(d[0], d[1], 0x5140), y = __byte_perm(d[2], d[3], 0x5140);
+                w0[j][s] = __byte_perm(x, y, 0x5410);
+                w1[j][s] = __byte_perm(x, y, 0x7632);
+                w2[j][s] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+            }
         }
         // B fragments: lane (column g, position quad t or t + 4) takes the digit words that lane (quad, query) holds
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-            const int from = 4 * (t + 4 * half) + (g >> 1);
+        for (int j = 0; j < ST; ++j)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                const uint32_t hi = __shfl_sync(0xffffffffu, w2[s], from), mid = __shfl_sync(0xffffffffu, w1[s], from);
-                bw[s][half] = (g & 1) ? mid : hi;
+            for (int half = 0; half < 2; ++half) {
+                const int from = 4 * (t + 4 * half) + (g >> 1);
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const uint32_t hi = __shfl_sync(0xffffffffu, w2[j][s], from), mid = __shfl_sync(0xffffffffu, w1[j][s], from);
+                    bw[j][s][half] = (g & 1) ? mid : hi;
+                }
+                const uint32_t lo = __shfl_sync(0xffffffffu, w0[j][0], from);
+                const uint32_t lo2 = NS == 2 ? __shfl_sync(0xffffffffu, w0[j][NS - 1], from) : 0u;
+                bw[j][NS][half] = (g & 1) ? lo2 : lo;
             }
-            const uint32_t lo = __shfl_sync(0xffffffffu, w0[0], from);
-            const uint32_t lo2 = NS == 2 ? __shfl_sync(0xffffffffu, w0[NS - 1], from) : 0u;
-            bw[NS][half] = (g & 1) ? lo2 : lo;
-        }
+        int acc[2 * VW][NT][4];                 // values 2 x (rows g) and 2 x + 1 (rows g + 8) of this lane
 #pragma unroll
-        for (int wd = 0; wd < VW; ++wd) {
-            uint32_t a[2][4];                   // [quad half][value 4 wd + r]: four positions each
+        for (int j = 0; j < ST; ++j) {
+            uint32_t v[8][VW];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint32_t x0 = v[4 * q][wd], x1 = v[4 * q + 1][wd], x2 = v[4 * q + 2][wd], x3 = v[4 * q + 3][wd];
-                const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
-                const uint32_t p2 = __byte_perm(x2, x3, 0x5140), p3 = __byte_perm(x2, x3, 0x7362);
-                a[q][0] = __byte_perm(p0, p2, 0x5410);
-                a[q][1] = __byte_perm(p0, p2, 0x7632);
-                a[q][2] = __byte_perm(p1, p3, 0x5410);
-                a[q][3] = __byte_perm(p1, p3, 0x7632);
+            for (int i = 0; i < 8; ++i) {
+                const int row = 4 * t + (i & 3) + 16 * (i >> 2);
+                if constexpr (VW == 4) {
+                    const uint4 x = *reinterpret_cast<const uint4*>(values + j * Half<HD>::kBytes + Half<HD>::value_at(row, g));
+                    v[i][0] = x.x; v[i][1] = x.y; v[i][2] = x.z; v[i][3] = x.w;
+                } else {
+                    const uint2 x = *reinterpret_cast<const uint2*>(values + j * Half<HD>::kBytes + Half<HD>::value_at(row, g >> 1) + 8 * (g & 1));
+                    v[i][0] = x.x; v[i][1] = x.y;
+                }
             }
 #pragma unroll
-            for (int pr = 0; pr < 2; ++pr) {    // values 4 wd + 2 pr (rows g) and 4 wd + 2 pr + 1 (rows g + 8)
-                int acc[NT][4];
+            for (int wd = 0; wd < VW; ++wd) {
+                uint32_t a[2][4];               // [quad half][value 4 wd + r]: four positions each
 #pragma unroll
-                for (int n = 0; n < NT; ++n) mma_first(acc[n], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[n][0], bw[n][1]);
+                for (int q = 0; q < 2; ++q) {
+                    const uint32_t x0 = v[4 * q][wd], x1 = v[4 * q + 1][wd], x2 = v[4 * q + 2][wd], x3 = v[4 * q + 3][wd];
+                    const uint32_t p0 = __byte_perm(x0, x1, 0x5140), p1 = __byte_perm(x0, x1, 0x7362);
+                    const uint32_t p2 = __byte_perm(x2, x3, 0x5140), p3 = __byte_perm(x2, x3, 0x7362);
+                    a[q][0] = __byte_perm(p0, p2, 0x5410);
+                    a[q][1] = __byte_perm(p0, p2, 0x7632);
+                    a[q][2] = __byte_perm(p1, p3, 0x5410);
+                    a[q][3] = __byte_perm(p1, p3, 0x7632);
+                }
 #pragma unroll
-                for (int s = 0; s < NS; ++s)
+                for (int pr = 0; pr < 2; ++pr)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        float& out = o[s][4 * wd + 2 * pr + e];
-                        out = fmaf(out, corr[s], join_digits(acc[s][2 * e], acc[s][2 * e + 1], acc[NS][2 * e + s]) * unit[s]);
+                    for (int n2 = 0; n2 < NT; ++n2) {
+                        if (j == 0) mma_first(acc[2 * wd + pr][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
+                        else mma_next(acc[2 * wd + pr][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
                     }
             }
         }
+#pragma unroll
+        for (int x = 0; x < 2 * VW; ++x)
+#pragma unroll
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float& out = o[s][2 * x + e];
+                    out = fmaf(join_digits(acc[x][s][2 * e], acc[x][s][2 * e + 1], acc[x][NS][2 * e + s]), unit[s], out);
+                }
     }
-    // tiles t0, t0 + stride, ... below t1 of the rows at kc / vc; the first one's loads may be under way (`loaded`)
-    __device__ __forceinline__ void run(const int8_t* kc, const float* ksc, const int8_t* vc, const float* vsc, int t0, int t1, int stride) {
-        for (; t0 < t1; t0 += stride) {
-            float sc[NS][4];
-            scores(sc, t0, t1);
-            const bool more = t1 - t0 > stride;
-            if (more) load_k(kc, ksc, t0 + stride, t1);       // on their way while this tile's values are added up
-            accumulate(sc, t0, t1);
-            if (more) load_v(vc, vsc, t0 + stride, t1);
-        }
-    }
-    // (max, sum, value) of every query into sm_ml[NQ][2], sm_o[NQ][HD]
-    __device__ __forceinline__ void store(float* sm_ml, float* sm_o) {
+    // (reference, sum, value) of the first nq queries into to_ml[NQ][2], to_o[NQ][HD]
+    __device__ __forceinline__ void store(float* to_ml, float* to_o, int nq = NQ) {
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) l[s] += __shfl_xor_sync(0xffffffffu, l[s], d);
             const int q = t + 4 * s;
-            if (g == 0) { sm_ml[2 * q] = m[s]; sm_ml[2 * q + 1] = l[s]; }
+            if (q >= nq) continue;
+            if (g == 0) { to_ml[2 * q] = m[s]; to_ml[2 * q + 1] = l[s]; }
 #pragma unroll
             for (int j = 0; j < VB; j += 4)
-                *reinterpret_cast<float4*>(sm_o + q * HD + VB * g + j) = make_float4(o[s][j], o[s][j + 1], o[s][j + 2], o[s][j + 3]);
+                *reinterpret_cast<float4*>(to_o + q * HD + VB * g + j) = make_float4(o[s][j], o[s][j + 1], o[s][j + 2], o[s][j + 3]);
         }
     }
 };
 
-// One warp, one row of HD values (VEC consecutive per lane), rotated if `turn`.
+// One warp rotates a row of HD values, VEC consecutive per lane: lane l < 16 holds the first ones of the pairs of lane l + 16.
 template <int HD>
-__device__ __forceinline__ void load_row(float (&v)[HD / 32], const float* row, const float* cos_row, const float* sin_row, bool turn, int lane) {
+__device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos_row, const float* sin_row, int lane) {
     constexpr int VEC = HD / 32;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) v[j] = row[lane * VEC + j];
-    if (!turn) return;
 #pragma unroll
     for (int j = 0; j < VEC; ++j) {
         const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
@@ -424,22 +507,27 @@ __device__ __forceinline__ void query_digits(const float (&v)[HD / 32], uint8_t*
     if (lane == 0) *unit = top >= 0x7F800000u ? CUDART_NAN_F : (fine ? __fmul_rn(__fdiv_rn(most, kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f);
 }
 
-// One warp quantizes a row into the cache.
+// One warp quantizes a row: its lane's codes (HD / 32 bytes) and the scale.
 template <int HD>
-__device__ __forceinline__ void append_row(const float (&v)[HD / 32], int8_t* codes, float* scale, int lane) {
-    constexpr int VEC = HD / 32;
-    float top = 1e-8f;
+struct HeldRow {
+    uint32_t codes;
+    float scale;
+    __device__ __forceinline__ void make(const float (&v)[HD / 32]) {
+        float top = 1e-8f;
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) top = absmax_step(top, v[j]);
-    top = warp_max(top);
-    const float inv = __fdiv_rn(127.0f, top);
-    if constexpr (VEC == 4)
-        *reinterpret_cast<char4*>(codes + lane * 4) = make_char4(quantize_code<127, -127>(v[0], inv), quantize_code<127, -127>(v[1], inv),
-                                                                 quantize_code<127, -127>(v[2], inv), quantize_code<127, -127>(v[3], inv));
-    else
-        *reinterpret_cast<char2*>(codes + lane * 2) = make_char2(quantize_code<127, -127>(v[0], inv), quantize_code<127, -127>(v[1], inv));
-    if (lane == 0) *scale = __fdiv_rn(top, 127.0f);
-}
+        for (int j = 0; j < HD / 32; ++j) top = absmax_step(top, v[j]);
+        top = warp_max(top);
+        const float inv = __fdiv_rn(127.0f, top);
+        codes = 0;
+#pragma unroll
+        for (int j = 0; j < HD / 32; ++j) codes |= (static_cast<uint32_t>(quantize_code<127, -127>(v[j], inv)) & 0xFFu) << (8 * j);
+        scale = __fdiv_rn(top, 127.0f);
+    }
+    __device__ __forceinline__ void put(void* row) const {               // row: where the lane's codes go
+        if constexpr (HD == 128) *static_cast<uint32_t*>(row) = codes;
+        else *static_cast<uint16_t*>(row) = static_cast<uint16_t>(codes);
+    }
+};
 
 struct DecodeArgs {
     const float* qkv;
@@ -455,9 +543,11 @@ struct DecodeArgs {
     int64_t out_stride;
     int pmode, nmain, nlow;
     uint8_t* planes;
-    const float* part_ml;              // prefix partial results [kv head][row][split][2] and [...][HD]
-    const float* part_o;
-    int parts;
+    float* part_ml;                    // partial results of the prefix: [kv head][row][split][2] and [...][HD]
+    float* part_o;
+    int parts;                         // splits of the prefix, 0: none
+    float* flat_ml;                    // partial results of attn_flat_int8_kernel: [slot][NQ][2] and [slot][NQ][HD]
+    float* flat_o;
 };
 
 __device__ __forceinline__ int64_t prefix_rows(const DecodeArgs& a) {
@@ -466,9 +556,7 @@ __device__ __forceinline__ int64_t prefix_rows(const DecodeArgs& a) {
     return p < 0 ? 0 : (p > a.first.max_seq ? a.first.max_seq : p);
 }
 
-constexpr int kWarps = 8;
-
-// Joins `n` partial results (max, sum at ml[2 i stride_ml], value at o[i * stride_o]) of one output value into (M, L, A)
+// Joins partial results (maximum, sum, value) of one output value
 struct Joined {
     float M, L, A;
 };
@@ -480,132 +568,491 @@ __device__ __forceinline__ void join_part(Joined& j, float m, float l, float a) 
     j.M = mn;
 }
 
-// grid (batch * kv heads, query blocks, S) in clusters of S along z: the S CTAs of a cluster split the positions of one (sequence,
-// kv head); the warp that owns the last position appends the new token's row first.  Warps are joined through shared memory and
-// CTAs through distributed shared memory, head g by CTA g % S.
+// The rows a new token brings to a kv head, held by one warp.
+template <int HD>
+struct NewRows {
+    HeldRow<HD> k, v;
+    __device__ __forceinline__ void make(const DecodeArgs& a, int b, int hk, const float* cos_row, const float* sin_row, int lane) {
+        constexpr int VEC = HD / 32;
+        const float* row = a.qkv + b * a.qkv_stride + lane * VEC;
+        float x[VEC], y[VEC];
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) {
+            x[j] = row[static_cast<int64_t>(a.n_heads + hk) * HD + j];
+            y[j] = row[static_cast<int64_t>(a.n_heads + a.n_kv + hk) * HD + j];
+        }
+        rotate_row<HD>(x, cos_row, sin_row, lane);
+        k.make(x);
+        v.make(y);
+    }
+    __device__ __forceinline__ void append(const DecodeArgs& a, int64_t row, int lane) const {
+        k.put(a.own.kc + row * HD + lane * (HD / 32));
+        v.put(a.own.vc + row * HD + lane * (HD / 32));
+        if (lane == 0) { a.own.ks[row] = k.scale; a.own.vs[row] = v.scale; }
+    }
+    // into row r of a half tile whose copy of the row is older
+    template <bool KEYS>
+    __device__ __forceinline__ void bring_in(uint8_t* half, int r, int lane) const {
+        const HeldRow<HD>& h = KEYS ? k : v;
+        const int byte = lane * (HD / 32);
+        h.put(half + Half<HD>::template at<KEYS>(r, byte >> 4) + (byte & 15));
+        if (lane == 0) *reinterpret_cast<float*>(half + Half<HD>::kScales + 4 * r) = h.scale;
+        __syncwarp();
+    }
+};
+
+// Finishes output value d of query head h of sequence b: the prefix's partial results, the division.
+template <int HD>
+__device__ __forceinline__ float finish(const DecodeArgs& a, Joined j, int b, int h, int d, bool live) {
+    const int G = a.n_heads / a.n_kv, hk = h / G;
+    if (live) {
+        const int64_t p0 = (static_cast<int64_t>(hk) * a.batch * G + static_cast<int64_t>(b) * G + h - hk * G) * a.parts;
+        for (int p = 0; p < a.parts; ++p) join_part(j, a.part_ml[2 * (p0 + p)], a.part_ml[2 * (p0 + p) + 1], a.part_o[(p0 + p) * HD + d]);
+    }
+    const float o = j.L == 0.f ? 0.f : j.A / j.L;
+    a.out[b * a.out_stride + static_cast<int64_t>(h) * HD + d] = o;
+    return o;
+}
+// One warp: a finished head as prepared activations of the [batch, n_heads * HD] matrix (a head is HD / 32 whole groups)
+template <int HD>
+__device__ __forceinline__ void prepare_head(const DecodeArgs& a, const float* head, int b, int h, int lane) {
+    const bool in = lane < HD / 8;
+    float v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = in ? head[lane * 8 + j] : 0.f;
+    const PreparedParts pp = prepared_parts(a.planes, static_cast<size_t>(a.n_heads) * (HD / 32), a.nmain, a.nlow);
+    convert_groups<kOrderNibble>(v, b, a.batch, static_cast<size_t>(h) * (HD / 32), a.pmode, a.nmain, a.nlow, 0.0625f, pp, in);
+}
+
+constexpr int kWarps = 8;
+// Short caches.  grid (batch * kv heads, query blocks, S) in clusters of S along z: the W warps of the S CTAs of a cluster take
+// the tiles of one (sequence, kv head) in turn, each through a ring of its own (nothing but warp barriers in the loop).
+// The warp of the last tile brings in the new token's row.  Warps are joined through shared memory; every CTA then stores its
+// partial result of head q into the shared memory of CTA q % S of the cluster, which finishes it.
+constexpr int kDecodeWarps = 4, kMaxSplits = 8;
 template <int HD, int NQ>
-__global__ void __launch_bounds__(kWarps * 32) attn_decode_int8_kernel(const DecodeArgs a) {
+struct DecodeShape {
+    static constexpr int ST = 128 / HD, kStep = ST * kTile, kGroup = ST * Half<HD>::kBytes;
+    static constexpr int kRecv = NQ + kMaxSplits - 1;                     // (head, sender) rows a CTA can receive: ceil(NQ / S) * S
+    static constexpr int kRing = kDecodeWarps * kGroups * kGroup;
+    static constexpr int kOuts = kDecodeWarps * NQ * HD * 4;
+    static constexpr int kQ = kRing > kOuts ? kRing : kOuts;              // the warps' outputs take the ring's place at the end
+    static constexpr int kPart = kQ + NQ * 3 * HD;
+    static constexpr int kSmall = kPart + kRecv * HD * 4;                 // units [NQ], received [kRecv][2], ml [warps][NQ][2]
+    static constexpr int kBytes = kSmall + (NQ + 2 * kRecv + 2 * kDecodeWarps * NQ) * 4;
+};
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(const DecodeArgs a) {
     namespace cg = cooperative_groups;
-    using Attn = WarpAttention<HD, NQ>;
-    __shared__ __align__(16) uint8_t sm_q[NQ * Attn::kQueryBytes];
-    __shared__ float sm_unit[NQ];
-    __shared__ float sm_ml[kWarps][NQ][2];
-    __shared__ __align__(16) float sm_o[kWarps][NQ][HD];
-    __shared__ float sm_part_ml[NQ][2];
-    __shared__ __align__(16) float sm_part[NQ][HD];
+    using Shape = DecodeShape<HD, NQ>;
+    constexpr int VEC = HD / 32, W = kDecodeWarps, ST = Shape::ST, STEP = Shape::kStep, GROUP = Shape::kGroup;
+    using Attn = WarpAttention<HD, NQ, ST>;
+    constexpr int QPW = (NQ + W - 1) / W;                                  // queries that a warp prepares
+    extern __shared__ __align__(128) uint8_t sm[];
+    uint8_t* sm_q = sm + Shape::kQ;
+    float* sm_part = reinterpret_cast<float*>(sm + Shape::kPart);         // [kRecv][HD]
+    float* sm_unit = reinterpret_cast<float*>(sm + Shape::kSmall);
+    float* sm_part_ml = sm_unit + NQ;                                     // [kRecv][2]
+    float* sm_ml = sm_part_ml + 2 * Shape::kRecv;
+    float* sm_o = reinterpret_cast<float*>(sm);                           // [W][NQ][HD]
+    cg::cluster_group cluster = cg::this_cluster();
+    const int S = gridDim.z;
     pdl_launch_dependents();
-    pdl_wait();
+    // Behind a prefix kernel only its partial results have to be waited for: that kernel lets this one start when
+    // everything older than the two is complete.
+    if (a.parts == 0) pdl_wait();
+    if (S > 1) cluster_arrive();                                           // every CTA is there when it comes to storing into it
     const int b = blockIdx.x / a.n_kv, hk = blockIdx.x - b * a.n_kv, G = a.n_heads / a.n_kv;
     const int q0 = blockIdx.y * NQ, nq = min(NQ, G - q0);             // this block's queries of the group
-    const int split = blockIdx.z, S = gridDim.z;
+    const int split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t pos = a.pos[b * a.pos_stride];
-    const bool live = pos >= 0 && pos < a.own.max_seq;
-    const int64_t P = prefix_rows(a);
-    const int n = live ? static_cast<int>(pos) + 1 : 0;
-    const int chunk = ((n + S - 1) / S + kTile - 1) / kTile * kTile;
-    const int t0 = min(static_cast<int64_t>(split) * chunk, static_cast<int64_t>(n)), t1 = min(static_cast<int64_t>(t0) + chunk, static_cast<int64_t>(n));
     const int64_t base = (static_cast<int64_t>(b) * a.n_kv + hk) * a.own.max_seq;
     const int8_t* kc = a.own.kc + base * HD;
     const int8_t* vc = a.own.vc + base * HD;
     const float* ks = a.own.ks + base;
     const float* vs = a.own.vs + base;
-    const float* row = a.qkv + b * a.qkv_stride;
+    uint8_t* ring = sm + warp * kGroups * GROUP;
+    const uint32_t ring_u = smem_u32(ring);
+    const int first = (split * W + warp) * STEP, stride = S * W * STEP, rows = static_cast<int>(a.own.max_seq);
+    // The first tile is asked for before the position is known: its rows lie inside the cache in any case.
+    request_group<HD, 32, ST, true>(ring_u, kc, ks, first, kTile, rows, lane);
+    cp_async_commit();
+    request_group<HD, 32, ST, false>(ring_u + GROUP, vc, vs, first, kTile, rows, lane);
+    cp_async_commit();
+    const float* row = a.qkv + b * a.qkv_stride + static_cast<int64_t>(hk * G + q0) * HD + lane * VEC;
+    float qv[QPW][VEC];
+#pragma unroll
+    for (int i = 0; i < QPW; ++i)
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) qv[i][j] = warp + i * W < nq ? row[(warp + i * W) * HD + j] : 0.f;
+    const int64_t pos = a.pos[b * a.pos_stride];
+    const bool live = pos >= 0 && pos < a.own.max_seq;
+    const int64_t P = prefix_rows(a);
+    const int n = live ? static_cast<int>(pos) + 1 : 0;
     const float* cos_row = a.cos_t + (live ? P + pos : 0) * (HD / 2);
     const float* sin_row = a.sin_t + (live ? P + pos : 0) * (HD / 2);
-
+    request_group<HD, 32, ST, true>(ring_u + 2 * GROUP, kc, ks, first + stride, kTile, n, lane);
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < QPW; ++i) {
+        rotate_row<HD>(qv[i], cos_row, sin_row, lane);
+        query_digits<HD>(qv[i], sm_q + (warp + i * W) * Attn::kQueryBytes, sm_unit + warp + i * W, lane);
+    }
+    // The warp that takes the last tile stores the new token's rows (in one query block of the group).
+    const bool owner = n > 0 && (n - 1) / STEP % (S * W) == split * W + warp;
+    NewRows<HD> fresh = {};
+    if (owner) {
+        fresh.make(a, b, hk, cos_row, sin_row, lane);
+        if (blockIdx.y == 0) fresh.append(a, base + pos, lane);
+    }
+    __syncthreads();
     Attn w;
     w.init(lane);
-    const int first = t0 + warp * kTile;
-    const bool owner = t1 == n && n > 0 && t1 > t0 && (n - 1 - t0) / kTile % kWarps == warp;
-    if (owner) {
-        // every query block of the group attends to the new row, so every one's owner writes it (the same bits)
-        float v[HD / 32];
-        load_row<HD>(v, row + static_cast<int64_t>(a.n_heads + hk) * HD, cos_row, sin_row, true, lane);
-        append_row<HD>(v, a.own.kc + (base + pos) * HD, a.own.ks + base + pos, lane);
-        load_row<HD>(v, row + static_cast<int64_t>(a.n_heads + a.n_kv + hk) * HD, cos_row, sin_row, false, lane);
-        append_row<HD>(v, a.own.vc + (base + pos) * HD, a.own.vs + base + pos, lane);
-        __syncwarp();
-    }
-    if (first < t1) {
-        w.load_k(kc, ks, first, t1);
-        w.load_v(vc, vs, first, t1);
-    }
-    for (int q = warp; q < NQ; q += kWarps) {
-        float v[HD / 32];
-        if (q < nq && live) {
-            load_row<HD>(v, row + static_cast<int64_t>(hk * G + q0 + q) * HD, cos_row, sin_row, true, lane);
-        } else {
-#pragma unroll
-            for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
-        }
-        query_digits<HD>(v, sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
-    }
-    __syncthreads();
     w.load_queries(sm_q, sm_unit);
-    w.run(kc, ks, vc, vs, first, t1, kWarps * kTile);
-    w.store(&sm_ml[warp][0][0], &sm_o[warp][0][0]);
+    int slot = 0;
+    for (int t = first; t < n; t += stride) {
+        int left[ST];
+#pragma unroll
+        for (int j = 0; j < ST; ++j) left[j] = n - t - j * kTile;
+        const bool last = owner && t + STEP >= n;
+        const int r = n - 1 - t;                                           // the new row's place in the last step
+        float sc[ST][Attn::NS][4];
+        cp_async_wait<kGroups - 1>();
+        __syncwarp();                                                      // the keys are there
+        uint8_t* group = ring + slot * GROUP;
+        if (last) fresh.template bring_in<true>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+        w.scores_of(sc, group, left);
+        __syncwarp();                                                      // everyone is through with them
+        request_group<HD, 32, ST, false>(ring_u + slot * GROUP, vc, vs, t + stride, kTile, n, lane);
+        cp_async_commit();
+        slot = next_slot(slot);
+        cp_async_wait<kGroups - 1>();
+        __syncwarp();
+        group = ring + slot * GROUP;
+        if (last) fresh.template bring_in<false>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+        w.accumulate(sc, group, left);
+        __syncwarp();
+        request_group<HD, 32, ST, true>(ring_u + slot * GROUP, kc, ks, t + 2 * stride, kTile, n, lane);
+        cp_async_commit();
+        slot = next_slot(slot);
+    }
+    cp_async_wait<0>();
+    __syncthreads();                                                       // the rings are free
+    w.store(sm_ml + warp * 2 * NQ, sm_o + warp * NQ * HD);
     __syncthreads();
-    for (int i = threadIdx.x; i < nq * HD; i += kWarps * 32) {
+    if (S > 1) cluster_wait();
+    for (int i = threadIdx.x; i < nq * HD; i += W * 32) {
         const int q = i / HD, d = i % HD;
         Joined j = {-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < kWarps; ++u) join_part(j, sm_ml[u][q][0], sm_ml[u][q][1], sm_o[u][q][d]);
-        sm_part[q][d] = j.A;
-        if (d == 0) { sm_part_ml[q][0] = j.M; sm_part_ml[q][1] = j.L; }
+        for (int u = 0; u < W; ++u) join_part(j, sm_ml[(u * NQ + q) * 2], sm_ml[(u * NQ + q) * 2 + 1], sm_o[(u * NQ + q) * HD + d]);
+        const int to = q % S, at = q / S * S + split;                      // row `at` of CTA `to`
+        cluster.map_shared_rank(sm_part, to)[at * HD + d] = j.A;
+        if (d == 0) {
+            float* ml = cluster.map_shared_rank(sm_part_ml, to) + 2 * at;
+            ml[0] = j.M;
+            ml[1] = j.L;
+        }
     }
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    const int64_t R = static_cast<int64_t>(a.batch) * G;
+    if (a.parts != 0) pdl_wait();
+    if (S > 1) {
+        cluster_arrive();
+        cluster_wait();
+    } else {
+        __syncthreads();
+    }
     for (int q = split; q < nq; q += S) {
+        const int h = hk * G + q0 + q;
         if (threadIdx.x < HD) {
             const int d = threadIdx.x;
             Joined j = {-CUDART_INF_F, 0.f, 0.f};
             for (int r = 0; r < S; ++r) {
-                const float* ml = cluster.map_shared_rank(&sm_part_ml[q][0], r);
-                join_part(j, ml[0], ml[1], cluster.map_shared_rank(&sm_part[q][0], r)[d]);
+                const int at = q / S * S + r;
+                join_part(j, sm_part_ml[2 * at], sm_part_ml[2 * at + 1], sm_part[at * HD + d]);
             }
-            if (live) {
-                const int64_t at = (hk * R + static_cast<int64_t>(b) * G + q0 + q) * a.parts;
-                for (int p = 0; p < a.parts; ++p) join_part(j, a.part_ml[2 * (at + p)], a.part_ml[2 * (at + p) + 1], a.part_o[(at + p) * HD + d]);
-            }
-            const float o = j.L == 0.f ? 0.f : j.A / j.L;
-            a.out[b * a.out_stride + static_cast<int64_t>(hk * G + q0 + q) * HD + d] = o;
-            sm_o[0][0][d] = o;
+            sm_o[d] = finish<HD>(a, j, b, h, d, live);
         }
         if (a.planes != nullptr) {
-            // the same values as prepared activations of the [batch, n_heads * HD] matrix: a head is HD / 32 whole groups
             __syncthreads();
-            if (warp == 0) {
-                const bool in = lane < HD / 8;
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = in ? sm_o[0][0][lane * 8 + j] : 0.f;
-                const PreparedParts pp = prepared_parts(a.planes, static_cast<size_t>(a.n_heads) * (HD / 32), a.nmain, a.nlow);
-                convert_groups<kOrderNibble>(v, b, a.batch, static_cast<size_t>(hk * G + q0 + q) * (HD / 32), a.pmode, a.nmain, a.nlow, 0.0625f, pp, in);
-            }
+            if (warp == 0) prepare_head<HD>(a, sm_o, b, h, lane);
             __syncthreads();
         }
     }
-    cluster.sync();                                                    // keeps shared memory alive until it has been read
+}
+
+// Long caches.  The steps (ST tiles) of all units (sequence, kv head, query block) in a row are dealt out evenly to all warps of
+// one CTA per SM: a warp works on one run of steps, which may end one unit and begin others, and writes a partial result for
+// each unit it touches.  How many steps a unit has follows from `pos` alone, so every warp (and the kernel that joins the
+// results) finds its place by itself: nothing is handed out at run time and the result does not depend on timing.
+// The partial result of warp w for unit u goes to slot w + u: from one part of the row to the next w or u grows.
+constexpr int kSms = 148;                     // what the plans count on, whatever the device has
+constexpr int kFlatWarpsPerSm = 8, kFlatWarps = kSms * kFlatWarpsPerSm;
+template <int HD, int NQ>
+struct FlatShape {
+    static constexpr int ST = HD == 128 ? 2 : 4, kStep = ST * kTile, kGroup = ST * Half<HD>::kBytes;
+    static constexpr int kQ = kFlatWarpsPerSm * kGroups * kGroup;         // digits [W][NQ][3][HD]
+    static constexpr int kSmall = kQ + kFlatWarpsPerSm * NQ * 3 * HD;     // units [W][NQ]
+    static constexpr int kBytes = kSmall + kFlatWarpsPerSm * NQ * 4;
+};
+// How the row of steps is dealt out.  Every warp works it out, from 32 sequences at a time.
+struct FlatPlan {
+    int total, per;
+    static __device__ __forceinline__ int steps(const DecodeArgs& a, int64_t b, int step) {
+        const int64_t pos = a.pos[b * a.pos_stride];
+        return pos >= 0 && pos < a.own.max_seq ? static_cast<int>(pos / step) + 1 : 0;
+    }
+    // steps of all sequences (for one head and query block), and of those in front of sequence b
+    __device__ __forceinline__ int make(const DecodeArgs& a, int units_per_seq, int b, int step, int lane) {
+        int all = 0, front = 0;
+        for (int i = lane; i < a.batch; i += 32) {
+            const int t = steps(a, i, step);
+            all += t;
+            front += i < b ? t : 0;
+        }
+        total = __reduce_add_sync(0xffffffffu, all) * units_per_seq;
+        per = max((total + kFlatWarps - 1) / kFlatWarps, 1);
+        return __reduce_add_sync(0xffffffffu, front);
+    }
+};
+template <int HD, int NQ>
+__global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(const DecodeArgs a, int blocks) {
+    using Shape = FlatShape<HD, NQ>;
+    constexpr int ST = Shape::ST, VEC = HD / 32, STEP = Shape::kStep;
+    using Attn = WarpAttention<HD, NQ, ST>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    pdl_launch_dependents();
+    if (a.parts == 0) pdl_wait();                                          // else at the end: see attn_decode_int8_kernel
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.n_heads / a.n_kv, units_per_seq = a.n_kv * blocks;
+    const int gw = blockIdx.x * kFlatWarpsPerSm + warp;
+    uint8_t* ring = sm + warp * kGroups * Shape::kGroup;
+    uint8_t* sm_q = sm + Shape::kQ + warp * NQ * Attn::kQueryBytes;
+    float* sm_unit = reinterpret_cast<float*>(sm + Shape::kSmall) + warp * NQ;
+    const uint32_t ring_u = smem_u32(ring);
+    FlatPlan plan;
+    plan.make(a, units_per_seq, 0, STEP, lane);
+    const int64_t lo = static_cast<int64_t>(gw) * plan.per;
+    int left = static_cast<int>(min(static_cast<int64_t>(plan.per), plan.total - lo));
+    if (left > 0) {
+        // the sequence, unit and step this warp's run begins with
+        int b = 0, before = 0, T = 0;
+        for (int b0 = 0; b0 < a.batch; b0 += 32) {
+            const int mine = b0 + lane < a.batch ? FlatPlan::steps(a, b0 + lane, STEP) * units_per_seq : 0;
+            int up = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int x = __shfl_up_sync(0xffffffffu, up, d);
+                if (lane >= d) up += x;
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, before + up > lo);
+            if (past) {
+                const int at = __ffs(past) - 1;
+                T = __shfl_sync(0xffffffffu, mine, at) / units_per_seq;
+                before += __shfl_sync(0xffffffffu, up - mine, at);
+                b = b0 + at;
+                break;
+            }
+            before += __shfl_sync(0xffffffffu, up, 31);
+        }
+        if (T == 0) left = 0;                                              // cannot be, unless somebody writes `pos` meanwhile
+        T = max(T, 1);
+        const int off = static_cast<int>(lo - before);
+        // A place in the row of steps: step s of T of unit j of sequence b, which has n positions
+        struct Place {
+            int b, j, s, T, n;
+        };
+        auto positions = [&](int seq) { return static_cast<int>(a.pos[seq * a.pos_stride]) + 1; };
+        auto advance = [&](Place& p) {                                     // only called while the run goes on: there is a next step
+            if (++p.s < p.T) return;
+            p.s = 0;
+            if (++p.j < units_per_seq) return;
+            p.j = 0;
+            do { p.T = FlatPlan::steps(a, ++p.b, STEP); } while (p.T == 0 && p.b + 1 < a.batch);
+            p.n = positions(p.b);
+        };
+        Place use = {b, off / T, off % T, T, positions(b)}, ask = use;
+        int to_ask = left;                                                 // steps whose values have not been asked for
+        int slot_ask = 0;
+        auto request = [&](bool keys) {
+            if (to_ask > 0) {
+                const int64_t base = (static_cast<int64_t>(ask.b) * a.n_kv + ask.j / blocks) * a.own.max_seq;
+                const uint32_t dst = ring_u + slot_ask * Shape::kGroup;
+                if (keys) {
+                    request_group<HD, 32, ST, true>(dst, a.own.kc + base * HD, a.own.ks + base, ask.s * STEP, kTile, ask.n, lane);
+                } else {
+                    request_group<HD, 32, ST, false>(dst, a.own.vc + base * HD, a.own.vs + base, ask.s * STEP, kTile, ask.n, lane);
+                    if (--to_ask > 0) advance(ask);
+                }
+            }
+            cp_async_commit();
+            slot_ask = next_slot(slot_ask);
+        };
+        request(true);
+        request(false);
+        request(true);
+        Attn w;
+        NewRows<HD> fresh = {};
+        bool begin = true;
+        int slot = 0;
+        for (; left > 0; --left) {
+            const int hk = use.j / blocks, qb = use.j - hk * blocks, q0 = qb * NQ, nq = min(NQ, G - q0);
+            const bool end = use.s + 1 == use.T;                           // of the unit
+            if (begin) {
+                const int64_t turn = (prefix_rows(a) + use.n - 1) * (HD / 2);
+                const float* row = a.qkv + use.b * a.qkv_stride + static_cast<int64_t>(hk * G + q0) * HD + lane * VEC;
+                float qv[NQ][VEC];
+#pragma unroll
+                for (int q = 0; q < NQ; ++q)
+#pragma unroll
+                    for (int j = 0; j < VEC; ++j) qv[q][j] = q < nq ? row[q * HD + j] : 0.f;
+#pragma unroll
+                for (int q = 0; q < NQ; ++q) {
+                    rotate_row<HD>(qv[q], a.cos_t + turn, a.sin_t + turn, lane);
+                    query_digits<HD>(qv[q], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
+                }
+                if (use.s + left >= use.T) {                               // the run holds the unit's last step
+                    fresh.make(a, use.b, hk, a.cos_t + turn, a.sin_t + turn, lane);
+                    if (qb == 0) fresh.append(a, (static_cast<int64_t>(use.b) * a.n_kv + hk) * a.own.max_seq + use.n - 1, lane);
+                }
+                __syncwarp();
+                w.init(lane);
+                w.load_queries(sm_q, sm_unit);
+                __syncwarp();                                              // everyone has read the digits
+                begin = false;
+            }
+            int in[ST];
+#pragma unroll
+            for (int j = 0; j < ST; ++j) in[j] = use.n - use.s * STEP - j * kTile;
+            const int r = (use.n - 1) % STEP;                              // the new row's place in the last step
+            float sc[ST][Attn::NS][4];
+            cp_async_wait<kGroups - 1>();
+            __syncwarp();                                                  // the keys are there
+            uint8_t* group = ring + slot * Shape::kGroup;
+            if (end) fresh.template bring_in<true>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+            w.scores_of(sc, group, in);
+            __syncwarp();                                                  // everyone is through with them
+            request(false);
+            slot = next_slot(slot);
+            cp_async_wait<kGroups - 1>();
+            __syncwarp();
+            group = ring + slot * Shape::kGroup;
+            if (end) fresh.template bring_in<false>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+            w.accumulate(sc, group, in);
+            __syncwarp();
+            request(true);
+            slot = next_slot(slot);
+            if (end || left == 1) {
+                const int64_t to = gw + static_cast<int64_t>(use.b) * units_per_seq + use.j;
+                w.store(a.flat_ml + to * NQ * 2, a.flat_o + to * NQ * HD, nq);
+                begin = true;
+            }
+            if (left > 1) advance(use);
+        }
+    }
+    cp_async_wait<0>();
+    if (a.parts != 0) pdl_wait();
+}
+
+// Joins the partial results of attn_flat_int8_kernel (and of a prefix).  WIDE: a block per (sequence, query head), whose warps take
+// the slots in turn; else a warp per (sequence, query head).  A lane holds HD / 32 values.  Where the slots are follows from
+// `pos`, which is older than the kernel in front: that is worked out before its results are waited for.
+template <int HD, int NQ, bool WIDE>
+__global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const DecodeArgs a, int blocks) {
+    constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, BY = WIDE ? kWarps : 1, U = 6;
+    __shared__ float sm_ml[kWarps][2];
+    __shared__ __align__(16) float sm_o[kWarps][HD];
+    pdl_launch_dependents();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.n_heads / a.n_kv, units_per_seq = a.n_kv * blocks;
+    const int64_t bh = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    const bool there = bh < static_cast<int64_t>(a.batch) * a.n_heads;
+    const int b = there ? static_cast<int>(bh / a.n_heads) : 0, h = there ? static_cast<int>(bh - static_cast<int64_t>(b) * a.n_heads) : 0;
+    const int hk = h / G, g = h - hk * G, j = hk * blocks + g / NQ;
+    FlatPlan plan;
+    const int front = plan.make(a, units_per_seq, b, STEP, lane) * units_per_seq, T = FlatPlan::steps(a, b, STEP);
+    const int start = front + j * T, w0 = start / plan.per, w1 = T > 0 ? (start + T - 1) / plan.per : w0 - 1;
+    const int64_t unit = static_cast<int64_t>(b) * units_per_seq + j;
+    float m = -CUDART_INF_F, l = 0.f, o[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+    pdl_wait();
+    for (int w = w0 + (WIDE ? warp : 0); w <= w1; w += U * BY) {
+        float pm[U], pl[U], po[U][VEC];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const bool in = w + u * BY <= w1;
+            const int64_t at = (unit + (in ? w + u * BY : w)) * NQ + g % NQ;
+            pm[u] = in ? a.flat_ml[2 * at] : -CUDART_INF_F;
+            pl[u] = in ? a.flat_ml[2 * at + 1] : 0.f;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) po[u][i] = in ? a.flat_o[at * HD + lane * VEC + i] : 0.f;
+        }
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
+        const float x = m == mn ? 1.0f : exp2_approx(m - mn);
+        l *= x;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) o[i] *= x;
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const float y = pm[u] == mn ? 1.0f : exp2_approx(pm[u] - mn);
+            l = fmaf(pl[u], y, l);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o[i] = fmaf(po[u][i], y, o[i]);
+        }
+        m = mn;
+    }
+    if constexpr (WIDE) {
+        if (lane == 0) { sm_ml[warp][0] = m; sm_ml[warp][1] = l; }
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = o[i];
+        __syncthreads();
+        if (threadIdx.x < HD) {
+            const int d = threadIdx.x;
+            Joined t = {-CUDART_INF_F, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < kWarps; ++u) join_part(t, sm_ml[u][0], sm_ml[u][1], sm_o[u][d]);
+            sm_o[0][d] = finish<HD>(a, t, b, h, d, T > 0);
+        }
+        if (a.planes == nullptr) return;
+        __syncthreads();
+        if (warp == 0) prepare_head<HD>(a, &sm_o[0][0], b, h, lane);
+    } else {
+        if (!there) return;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = finish<HD>(a, Joined{m, l, o[i]}, b, h, lane * VEC + i, T > 0);
+        __syncwarp();
+        if (a.planes != nullptr) prepare_head<HD>(a, &sm_o[warp][0], b, h, lane);
+    }
 }
 
 // Partial attention of every sequence's queries to the shared prefix.  grid (kv heads, splits of the prefix, blocks of 8 QW rows),
-// the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; QW warps of a block take
-// the same positions (their loads meet in L1) and the KW = 8 / QW groups of warps take alternate tiles.
-template <int HD>
-__global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const DecodeArgs a, int QW, float* __restrict__ part_ml, float* __restrict__ part_o) {
-    constexpr int NQ = 8;
-    using Attn = WarpAttention<HD, NQ>;
-    constexpr int kDigits = kWarps * NQ * Attn::kQueryBytes, kOuts = kWarps * NQ * HD * 4;
-    __shared__ __align__(16) uint8_t sm[kDigits > kOuts ? kDigits : kOuts];      // the queries' digits, then the warps' outputs
-    __shared__ float sm_unit[kWarps * NQ];
-    __shared__ float sm_ml[kWarps][NQ][2];
-    pdl_launch_dependents();
+// the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; the QW warps of a group
+// take the same tiles, which they fetch together into the group's ring, and the KW = 8 / QW groups take alternate tiles.
+template <int HD, int QW>
+struct PrefixShape {
+    static constexpr int NQ = 8, KW = kWarps / QW;
+    static constexpr int ST = (QW == 1 ? 2 : 4) * (128 / HD) > 4 ? 4 : (QW == 1 ? 2 : 4) * (128 / HD);
+    static constexpr int kGroup = ST * Half<HD>::kBytes, kRing = KW * kGroups * kGroup;
+    static constexpr int kOuts = kWarps * NQ * HD * 4;
+    static constexpr int kQ = kRing > kOuts ? kRing : kOuts;
+    static constexpr int kSmall = kQ + QW * NQ * 3 * HD;                  // units [QW][NQ], ml [warps][NQ][2]
+    static constexpr int kBytes = kSmall + (QW * NQ + kWarps * NQ * 2) * 4;
+};
+template <int HD, int QW>
+__global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const DecodeArgs a) {
+    using Shape = PrefixShape<HD, QW>;
+    constexpr int NQ = Shape::NQ, KW = Shape::KW, ST = Shape::ST;
+    using Attn = WarpAttention<HD, NQ, ST>;
+    extern __shared__ __align__(128) uint8_t sm[];
+    uint8_t* sm_q = sm + Shape::kQ;
+    float* sm_unit = reinterpret_cast<float*>(sm + Shape::kSmall);
+    float* sm_ml = sm_unit + QW * NQ;
+    float* sm_o = reinterpret_cast<float*>(sm);
     pdl_wait();
+    pdl_launch_dependents();                                                // behind the wait: see attn_decode_int8_kernel
     const int hk = blockIdx.x, split = blockIdx.y, splits = gridDim.y, G = a.n_heads / a.n_kv;
     const int64_t R = static_cast<int64_t>(a.batch) * G, r0 = static_cast<int64_t>(blockIdx.z) * QW * NQ;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, KW = kWarps / QW, qg = warp % QW, kw = warp / QW;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, qg = warp % QW, kw = warp / QW, in_group = threadIdx.x % (QW * 32);
     const int n = static_cast<int>(prefix_rows(a));
     const int chunk = ((n + splits - 1) / splits + kTile - 1) / kTile * kTile;
     const int t0 = min(static_cast<int64_t>(split) * chunk, static_cast<int64_t>(n)), t1 = min(static_cast<int64_t>(t0) + chunk, static_cast<int64_t>(n));
@@ -614,44 +1061,80 @@ __global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const Dec
     const int8_t* vc = a.first.vc + base * HD;
     const float* ks = a.first.ks + base;
     const float* vs = a.first.vs + base;
-    Attn w;
-    w.init(lane);
+
+    uint8_t* ring = sm + kw * kGroups * Shape::kGroup;
+    const uint32_t ring_u = smem_u32(ring);
+    constexpr int BETWEEN = KW * kTile, STRIDE = ST * BETWEEN;              // tiles of a step, steps
+    auto request = [&](int slot, int t, bool keys) {
+        const uint32_t dst = ring_u + slot * Shape::kGroup;
+        if (keys) request_group<HD, QW * 32, ST, true>(dst, kc, ks, t, BETWEEN, t1, in_group);
+        else request_group<HD, QW * 32, ST, false>(dst, vc, vs, t, BETWEEN, t1, in_group);
+        cp_async_commit();
+    };
+    auto group_sync = [&] {
+        if constexpr (QW == 1) __syncwarp();
+        else named_barrier_sync(1 + kw, QW * 32);
+    };
     const int first = t0 + kw * kTile;
-    if (first < t1) {
-        w.load_k(kc, ks, first, t1);
-        w.load_v(vc, vs, first, t1);
-    }
-    for (int i = warp; i < QW * NQ; i += kWarps) {
-        const int64_t r = r0 + i;
+    request(0, first, true);
+    request(1, first, false);
+    request(2, first + STRIDE, true);
+    float v[QW][HD / 32];                                                   // this warp's rows: warp, warp + 8, ...
+#pragma unroll
+    for (int i = 0; i < QW; ++i) {
+        const int64_t r = r0 + warp + i * kWarps;
         const int64_t b = r < R ? r / G : 0;
         const int64_t pos = a.pos[b * a.pos_stride];
-        float v[HD / 32];
-        if (r < R && pos >= 0 && pos < a.own.max_seq) {
-            load_row<HD>(v, a.qkv + b * a.qkv_stride + (hk * G + r - b * G) * HD, a.cos_t + (n + pos) * (HD / 2), a.sin_t + (n + pos) * (HD / 2), true, lane);
-        } else {
+        const bool live = r < R && pos >= 0 && pos < a.own.max_seq;
+        const int64_t turn = (live ? n + pos : 0) * (HD / 2);
 #pragma unroll
-            for (int j = 0; j < HD / 32; ++j) v[j] = 0.f;
-        }
-        query_digits<HD>(v, sm + i * Attn::kQueryBytes, sm_unit + i, lane);
+        for (int j = 0; j < HD / 32; ++j) v[i][j] = live ? a.qkv[b * a.qkv_stride + (hk * G + r - b * G) * HD + lane * (HD / 32) + j] : 0.f;
+        rotate_row<HD>(v[i], a.cos_t + turn, a.sin_t + turn, lane);
+    }
+#pragma unroll
+    for (int i = 0; i < QW; ++i) {
+        const int q = warp + i * kWarps;
+        query_digits<HD>(v[i], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
     }
     __syncthreads();
-    w.load_queries(sm + qg * NQ * Attn::kQueryBytes, sm_unit + qg * NQ);
-    w.run(kc, ks, vc, vs, first, t1, KW * kTile);
-    __syncthreads();                                                    // everyone has read the digits
-    float* sm_o = reinterpret_cast<float*>(sm);
-    w.store(&sm_ml[warp][0][0], sm_o + warp * NQ * HD);
+    Attn w;
+    w.init(lane);
+    w.load_queries(sm_q + qg * NQ * Attn::kQueryBytes, sm_unit + qg * NQ);
+    int slot = 0;
+    for (int t = first; t < t1; t += STRIDE) {
+        int left[ST];
+#pragma unroll
+        for (int j = 0; j < ST; ++j) left[j] = t1 - t - j * BETWEEN;
+        float sc[ST][Attn::NS][4];
+        cp_async_wait<kGroups - 1>();
+        group_sync();                                                       // the keys are there
+        w.scores_of(sc, ring + slot * Shape::kGroup, left);
+        group_sync();                                                       // everyone is through with them
+        request(slot, t + STRIDE, false);
+        slot = next_slot(slot);
+        cp_async_wait<kGroups - 1>();
+        group_sync();
+        w.accumulate(sc, ring + slot * Shape::kGroup, left);
+        group_sync();
+        request(slot, t + 2 * STRIDE, true);
+        slot = next_slot(slot);
+    }
+    cp_async_wait<0>();
+    __syncthreads();                                                        // the rings are free
+    w.store(sm_ml + warp * 2 * NQ, sm_o + warp * NQ * HD);
     __syncthreads();
     for (int i = threadIdx.x; i < QW * NQ * HD; i += kWarps * 32) {
         const int q = i / HD, d = i % HD;
         if (r0 + q >= R) break;
         Joined j = {-CUDART_INF_F, 0.f, 0.f};
+#pragma unroll
         for (int u = 0; u < KW; ++u) {
-            const int wi = q / NQ + u * QW;
-            join_part(j, sm_ml[wi][q % NQ][0], sm_ml[wi][q % NQ][1], sm_o[(wi * NQ + q % NQ) * HD + d]);
+            const int at = (q / NQ + u * QW) * NQ + q % NQ;
+            join_part(j, sm_ml[2 * at], sm_ml[2 * at + 1], sm_o[at * HD + d]);
         }
-        const int64_t at = (hk * R + r0 + q) * splits + split;
-        part_o[at * HD + d] = j.A;
-        if (d == 0) { part_ml[2 * at] = j.M; part_ml[2 * at + 1] = j.L; }
+        const int64_t to = (hk * R + r0 + q) * splits + split;
+        a.part_o[to * HD + d] = j.A;
+        if (d == 0) { a.part_ml[2 * to] = j.M; a.part_ml[2 * to + 1] = j.L; }
     }
 }
 
@@ -673,8 +1156,7 @@ int check_cache_pointers(const sgqd_cache_int8* c) {
 CacheView view(const sgqd_cache_int8* c) { return CacheView{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->max_seq}; }
 
 // Splits of a shared prefix and rows per block of its kernel: a function of the sizes alone, so that the workspace's size is one
-// too.  148 SMs, one block each.
-constexpr int kPrefixBlocks = 148;
+// too: the plans count 148 SMs, whatever the device has.
 struct PrefixPlan {
     int qw, blocks, splits;
     int64_t rows;                        // (kv head, query row) pairs
@@ -685,8 +1167,8 @@ PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t hea
     const int64_t R = batch * (n_heads / n_kv);
     p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : (R <= 32 ? 4 : 8));
     p.blocks = static_cast<int>(ceil_div(R, 8 * p.qw));
-    const int64_t most = ceil_div(prefix_max, kTile * (kWarps / p.qw));              // a tile for every warp
-    int64_t s = kPrefixBlocks / (n_kv * p.blocks);
+    const int64_t most = ceil_div(prefix_max, kTile * (kWarps / p.qw));              // a tile for every group of warps
+    int64_t s = kSms / (n_kv * p.blocks);
     s = s < 1 ? 1 : (s > most ? most : s);
     p.splits = static_cast<int>(s > 65535 ? 65535 : s);
     p.rows = n_kv * R;
@@ -695,30 +1177,102 @@ PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t hea
     return p;
 }
 
+template <int HD, int QW>
+int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
+    static SmemOptIn opt_in;
+    constexpr int bytes = PrefixShape<HD, QW>::kBytes;
+    SGQ_CUDA_TRY(opt_in.ensure(attn_prefix_int8_kernel<HD, QW>, bytes));
+    const dim3 grid(static_cast<unsigned>(a.n_kv), static_cast<unsigned>(plan.splits), static_cast<unsigned>(plan.blocks));
+    SGQ_CUDA_TRY(launch_kernel(attn_prefix_int8_kernel<HD, QW>, grid, dim3(kWarps * 32), bytes, s, true, a));
+    return SGQ_OK;
+}
+template <int HD>
+int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
+    switch (plan.qw) {
+        case 1: return launch_prefix<HD, 1>(a, plan, s);
+        case 2: return launch_prefix<HD, 2>(a, plan, s);
+        case 4: return launch_prefix<HD, 4>(a, plan, s);
+        default: return launch_prefix<HD, 8>(a, plan, s);
+    }
+}
+
+// Which kernel reads the sequences' own rows.  `flat`: few units over long caches, where clusters cannot fill the device (one
+// sequence x 8 heads: 18.8 -> 15.4 us at 16384 positions, 110 -> 53 us at 131071); its second launch costs 3 us.
+struct DecodePlan {
+    int nq, blocks, splits;
+    int64_t units;                       // (sequence, kv head, query block)
+    bool flat;
+    size_t off_o, bytes;                 // of the flat kernel's partial results
+};
+DecodePlan decode_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_seq) {
+    DecodePlan p = {};
+    const int64_t G = n_heads / n_kv;
+    // four queries per warp where the group has no more: 2 column sets in the place of 3 and half the outputs in registers
+    p.nq = G <= 4 ? 4 : 8;
+    p.blocks = static_cast<int>(ceil_div(G, p.nq));
+    p.units = batch * n_kv * p.blocks;
+    const int64_t units = p.units, tiles = ceil_div(max_seq, kTile);
+    p.flat = units * kMaxSplits < 3 * kSms && units * tiles >= 16 * kSms && units * tiles < (1 << 30);
+    if (p.flat) {
+        const size_t slots = static_cast<size_t>(units + kFlatWarps);
+        p.off_o = (slots * p.nq * 8 + 255) / 256 * 256;
+        p.bytes = p.off_o + slots * p.nq * head_dim * 4;
+    }
+    // Splits: enough CTAs for sequences of unequal length to even out (about 1000, three of them per SM: batch 32 x 8 heads of up
+    // to 8192 positions 76 / 58 / 56 / 55 / 62 us with 1 / 2 / 3 / 4 / 8 splits), with two steps for each warp or, where the
+    // units do not fill the SMs, one (batch 8 x 16 heads, 576 positions: 9.0 / 12.7 us with 2 / 4; batch 5 x 4 heads of 64,
+    // up to 1500: 6.6 / 6.0 with 3 / 6).
+    const int64_t steps = ceil_div(max_seq, (128 / head_dim) * kTile);
+    int64_t S = (1000 + units / 2) / units;
+    const int64_t two = steps / (2 * kDecodeWarps), fill = 2 * kSms / units, one = ceil_div(steps, kDecodeWarps);
+    S = std::min(std::min(S, one), std::max(two, fill));
+    p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>(S, kMaxSplits), 1));
+    return p;
+}
+
 template <int HD, int NQ>
-int launch_decode(const DecodeArgs& a, int64_t batch, cudaStream_t s) {
-    const int G = a.n_heads / a.n_kv, blocks = (G + NQ - 1) / NQ;
-    const int64_t units = batch * a.n_kv * blocks;
-    // splits of the positions: a block per SM slot, at least a tile for each of its warps, at most the portable cluster size
-    int64_t S = 2 * static_cast<int64_t>(sm_count()) / units;
-    const int64_t most = ceil_div(a.own.max_seq, kTile * kWarps);
-    S = S > most ? most : S;
-    S = S > 8 ? 8 : (S < 1 ? 1 : S);
+int launch_decode(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
+    if (plan.flat) {
+        static SmemOptIn opt_in;
+        constexpr int bytes = FlatShape<HD, NQ>::kBytes;
+        SGQ_CUDA_TRY(opt_in.ensure(attn_flat_int8_kernel<HD, NQ>, bytes));
+        SGQ_CUDA_TRY(launch_kernel(attn_flat_int8_kernel<HD, NQ>, dim3(kSms), dim3(kFlatWarpsPerSm * 32), bytes, s, true, a, plan.blocks));
+        const int64_t heads = static_cast<int64_t>(a.batch) * a.n_heads;
+        // a head has about kFlatWarps / units slots: with more than a warp asks for at once, a block takes it
+        if (plan.units * 6 < kFlatWarps)
+            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, true>, dim3(static_cast<unsigned>(heads)), dim3(kWarps * 32), 0, s, true, a, plan.blocks));
+        else
+            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, false>, dim3(static_cast<unsigned>(ceil_div(heads, kWarps))), dim3(kWarps * 32), 0, s, true,
+                                       a, plan.blocks));
+        return SGQ_OK;
+    }
+    static SmemOptIn opt_in;
+    constexpr int bytes = DecodeShape<HD, NQ>::kBytes;
+    SGQ_CUDA_TRY(opt_in.ensure(attn_decode_int8_kernel<HD, NQ>, bytes));
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(static_cast<unsigned>(batch * a.n_kv), static_cast<unsigned>(blocks), static_cast<unsigned>(S));
-    cfg.blockDim = dim3(kWarps * 32);
+    cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.n_kv), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(plan.splits));
+    cfg.blockDim = dim3(kDecodeWarps * 32);
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = 1;
     attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = static_cast<unsigned>(S);
+    attr[0].val.clusterDim.z = static_cast<unsigned>(plan.splits);
     attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     SGQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_decode_int8_kernel<HD, NQ>, a));
     return SGQ_OK;
+}
+
+size_t decode_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_seq, int64_t prefix_max) {
+    if (batch <= 0 || batch > 0x7fffffff || n_heads <= 0 || n_heads > 65535 || n_kv <= 0 || n_heads % n_kv || max_seq <= 0 || max_seq > kMaxPositions ||
+        prefix_max < 0 || prefix_max > kMaxPositions || (head_dim != 64 && head_dim != 128))
+        return 0;
+    const size_t flat = decode_plan(batch, n_heads, n_kv, head_dim, max_seq).bytes;
+    return (flat + 255) / 256 * 256 + (prefix_max ? prefix_plan(batch, n_heads, n_kv, head_dim, prefix_max).bytes : 0);
 }
 
 int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table, int64_t table_rows,
@@ -745,33 +1299,38 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
         return bad(SGQ_ERR_ALIGNMENT, "qkv rows and tables must be 16-byte aligned");
     PreparedLayout L = {};
     if ((rc = check_prepared(prepared_out, prepared_bytes, batch, n_heads * hd, &L)) != SGQ_OK) return rc;
-    PrefixPlan plan = {};
+    const DecodePlan plan = decode_plan(batch, n_heads, kv, hd, cache->max_seq);
+    PrefixPlan first = {};
     if (prefix) {
-        plan = prefix_plan(batch, n_heads, kv, hd, prefix->max_seq);
-        if (plan.blocks > 65535) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
-        if (!workspace || workspace_bytes < plan.bytes || !aligned(workspace, 256)) return bad(SGQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
+        first = prefix_plan(batch, n_heads, kv, hd, prefix->max_seq);
+        if (first.blocks > 65535) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
     }
+    const size_t need = decode_workspace(batch, n_heads, kv, hd, cache->max_seq, prefix ? prefix->max_seq : 0);
+    if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
+        return bad(SGQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
+    if (batch * n_heads > 0x7fffffff) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
     if ((rc = check_device()) != SGQ_OK) return rc;
     DecodeArgs a = {};
     a.qkv = qkv; a.qkv_stride = qkv_stride; a.n_heads = static_cast<int>(n_heads); a.n_kv = static_cast<int>(kv); a.batch = static_cast<int>(batch);
     a.cos_t = cos_table; a.sin_t = sin_table; a.pos = pos; a.pos_stride = pos_stride; a.own = view(cache);
     a.out = out; a.out_stride = out_stride; a.pmode = L.mode; a.nmain = L.nmain; a.nlow = L.nlow; a.planes = static_cast<uint8_t*>(prepared_out);
+    uint8_t* ws = static_cast<uint8_t*>(workspace);
+    if (plan.flat) {
+        a.flat_ml = reinterpret_cast<float*>(ws);
+        a.flat_o = reinterpret_cast<float*>(ws + plan.off_o);
+    }
     if (prefix) {
+        uint8_t* at = ws + (plan.bytes + 255) / 256 * 256;
         a.first = view(prefix);
         a.prefix_len = prefix_len;
-        float* ml = static_cast<float*>(workspace);
-        float* o = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + plan.off_o);
-        const dim3 grid(static_cast<unsigned>(kv), static_cast<unsigned>(plan.splits), static_cast<unsigned>(plan.blocks));
-        if (hd == 128) SGQ_CUDA_TRY(launch_kernel(attn_prefix_int8_kernel<128>, grid, dim3(kWarps * 32), 0, s, true, a, plan.qw, ml, o));
-        else SGQ_CUDA_TRY(launch_kernel(attn_prefix_int8_kernel<64>, grid, dim3(kWarps * 32), 0, s, true, a, plan.qw, ml, o));
-        a.part_ml = ml;
-        a.part_o = o;
-        a.parts = plan.splits;
+        a.part_ml = reinterpret_cast<float*>(at);
+        a.part_o = reinterpret_cast<float*>(at + first.off_o);
+        a.parts = first.splits;
+        rc = hd == 128 ? launch_prefix<128>(a, first, s) : launch_prefix<64>(a, first, s);
+        if (rc != SGQ_OK) return rc;
     }
-    // four queries per warp where the group has no more: 2 column sets in the place of 3 and half the outputs in registers
-    const bool four = n_heads / kv <= 4;
-    if (hd == 128) return four ? launch_decode<128, 4>(a, batch, s) : launch_decode<128, 8>(a, batch, s);
-    return four ? launch_decode<64, 4>(a, batch, s) : launch_decode<64, 8>(a, batch, s);
+    if (hd == 128) return plan.nq == 4 ? launch_decode<128, 4>(a, plan, s) : launch_decode<128, 8>(a, plan, s);
+    return plan.nq == 4 ? launch_decode<64, 4>(a, plan, s) : launch_decode<64, 8>(a, plan, s);
 }
 
 }  // namespace
@@ -838,27 +1397,29 @@ int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_t batch,
     return SGQ_OK;
 }
 
-int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table,
-                          int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, float* out, int64_t out_stride,
-                          void* prepared_out, size_t prepared_bytes, void* stream) {
-    return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, nullptr, nullptr, out, out_stride, prepared_out,
-                       prepared_bytes, nullptr, 0, static_cast<cudaStream_t>(stream));
+size_t sgqd_attn_decode_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_seq) {
+    return decode_workspace(batch, n_heads, n_kv_heads, head_dim, max_seq, 0);
 }
 
-size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t prefix_max) {
-    if (batch <= 0 || batch > 0x7fffffff || n_heads <= 0 || n_heads > 65535 || n_kv_heads <= 0 || n_heads % n_kv_heads || prefix_max <= 0 ||
-        prefix_max > kMaxPositions || (head_dim != 64 && head_dim != 128))
-        return 0;
-    return prefix_plan(batch, n_heads, n_kv_heads, head_dim, prefix_max).bytes;
+int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table,
+                          int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, float* out, int64_t out_stride,
+                          void* prepared_out, size_t prepared_bytes, void* workspace, size_t workspace_bytes, void* stream) {
+    return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, nullptr, nullptr, out, out_stride,
+                       prepared_out, prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, int64_t max_seq,
+                                                    int64_t prefix_max) {
+    return prefix_max > 0 ? decode_workspace(batch, n_heads, n_kv_heads, head_dim, max_seq, prefix_max) : 0;
 }
 
 int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table, const float* sin_table,
-                                 int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache, const sgqd_cache_int8* prefix,
-                                 const int32_t* prefix_len, float* out, int64_t out_stride, void* prepared_out, size_t prepared_bytes,
-                                 void* workspace, size_t workspace_bytes, void* stream) {
+                                 int64_t table_rows, const int32_t* pos, int64_t pos_stride, const sgqd_cache_int8* cache,
+                                 const sgqd_cache_int8* prefix, const int32_t* prefix_len, float* out, int64_t out_stride, void* prepared_out,
+                                 size_t prepared_bytes, void* workspace, size_t workspace_bytes, void* stream) {
     if (!prefix) return bad(SGQ_ERR_NULL_POINTER, "prefix is NULL");
-    return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, prefix, prefix_len, out, out_stride, prepared_out,
-                       prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    return attn_decode(qkv, qkv_stride, n_heads, cos_table, sin_table, table_rows, pos, pos_stride, cache, prefix, prefix_len, out, out_stride,
+                       prepared_out, prepared_bytes, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

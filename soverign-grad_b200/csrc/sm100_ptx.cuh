@@ -199,6 +199,10 @@ __device__ __forceinline__ uint32_t cluster_cta_rank() {
 __device__ __forceinline__ void cluster_sync_all() {
     asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
+// The two halves of a cluster barrier, for warps that may be diverged: what was stored before an arrive, into the shared
+// memory of other CTAs too, is visible behind the wait.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire;" ::: "memory"); }
 // The address of the same object in CTA `rank` of the cluster.
 __device__ __forceinline__ uint32_t map_to_rank(const void* p, uint32_t rank) {
     uint32_t r;

@@ -547,18 +547,20 @@ struct DecodeOut {
     }
 };
 
-// attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared)
+// attn_decode_int8(qkv, cache, cos, sin, pos, n_heads, out, prepared, workspace)
 PyObject* attn_decode_int8(PyObject* const* a, Py_ssize_t n) {
-    if (n != 8) raise(PyExc_TypeError, "attn_decode_int8 takes eight arguments");
+    if (n != 9) raise(PyExc_TypeError, "attn_decode_int8 takes nine arguments");
     const Cache8 cache(a[1]);
     Rotary r(a[0], cache, a[2], a[3], a[4], a[5], true);
     const c10::cuda::CUDAGuard guard(r.qkv.t.device());
     r.readable();
     DecodeOut o(a[6], a[7], r);
+    const Scratch ws(a[8], sgqd_attn_decode_int8_workspace_bytes(cache.c.batch, r.heads, cache.c.n_kv_heads, cache.c.head_dim, cache.c.max_seq), r.qkv.t);
+    if (ws.buf.defined() && ws.buf.device() != r.qkv.t.device()) raise(PyExc_ValueError, "all tensors must be on one GPU");
     void* s = stream();
     check(without_gil([&] {
               return sgqd_attn_decode_int8(fptr(r.qkv.t), r.qkv.stride, r.heads, fptr(r.cos), fptr(r.sin), r.cos.size(0), r.pos.p, r.pos_stride(), &cache.c,
-                                           fptr(o.out), o.stride, o.p, o.bytes, s);
+                                           fptr(o.out), o.stride, o.p, o.bytes, ws.ptr, ws.bytes, s);
           }),
           "sgqd_attn_decode_int8");
     return o.result();
@@ -579,7 +581,8 @@ PyObject* attn_decode_prefix_int8(PyObject* const* a, Py_ssize_t n) {
     const c10::cuda::CUDAGuard guard(d);
     r.readable();
     DecodeOut o(a[8], a[9], r);
-    const Scratch ws(a[10], sgqd_attn_decode_prefix_int8_workspace_bytes(cache.c.batch, r.heads, cache.c.n_kv_heads, cache.c.head_dim, prefix.c.max_seq),
+    const Scratch ws(a[10], sgqd_attn_decode_prefix_int8_workspace_bytes(cache.c.batch, r.heads, cache.c.n_kv_heads, cache.c.head_dim, cache.c.max_seq,
+                                                                           prefix.c.max_seq),
                      r.qkv.t);
     if (ws.buf.defined() && ws.buf.device() != d) raise(PyExc_ValueError, "all tensors must be on one GPU");
     void* s = stream();

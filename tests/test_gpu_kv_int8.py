@@ -202,7 +202,24 @@ DECODE = [
     (1, 1, 1, 128, 1, [0]), (1, 1, 1, 64, 8, [7]), (2, 2, 2, 128, 64, [6, 0]), (1, 8, 1, 128, 70, [32]), (8, 16, 16, 128, 640, [129]),
     (3, 5, 5, 64, 333, [332, 0, 31]), (2, 12, 3, 64, 100, [63, 64]), (2, 10, 2, 128, 257, [255, 256]), (1, 14, 2, 64, 1000, [999]),
     (2, 32, 4, 128, 300, [299, 150]), (1, 16, 1, 128, 90, [33]), (1, 34, 2, 64, 50, [40]), (40, 32, 32, 64, 128, [100]),
-    (5, 4, 1, 128, 2051, [2050, -1, 17, 2051, 1024]), (1, 4, 2, 128, 9001, [9000]), (3, 24, 8, 128, 31, [-5, 30, 1])]
+    (5, 4, 1, 128, 2051, [2050, -1, 17, 2051, 1024]), (1, 4, 2, 128, 9001, [9000]), (3, 24, 8, 128, 31, [-5, 30, 1]), (37, 8, 8, 64, 512, [500]), (33, 16, 16, 128, 300, [255]),
+    (16, 8, 4, 128, 1500, [1499 - 99 * i for i in range(16)]), (9, 40, 8, 64, 700, [699, 64, 63, 128, 127, 0, 1, -1, 300])]
+
+
+# caches that may grow long (dealt out to all warps of the device): few and many positions in them, idle slots at every place
+LONG = [
+    (1, 4, 2, 128, 80000, [70001]), (1, 16, 16, 128, 9600, [0]), (3, 8, 8, 128, 7000, [6999, 63, 64]), (2, 32, 4, 64, 20000, [127, 19999]),
+    (5, 8, 8, 64, 2000, [-1, 1999, -1, 128, -1]), (2, 48, 4, 128, 19000, [300, 5000]), (37, 2, 1, 64, 5000, [500]), (2, 40, 2, 128, 16000, [15999, 0]),
+    (40, 4, 1, 128, 2000, [(51 * i) % 2003 - 2 for i in range(40)]), (4, 10, 2, 128, 20000, [-1, -1, -1, -1]), (33, 1, 1, 128, 3000, [255])]
+
+
+@pytest.mark.parametrize("B,heads,kv,dim,S,pos", LONG)
+def test_decode_over_long_caches(sgq, B, heads, kv, dim, S, pos):
+    assert sgq.lib.sgqd_attn_decode_int8_workspace_bytes(B, heads, kv, dim, S) > 0
+    got = run_decode(sgq, B, heads, kv, dim, S, pos)
+    for b, p in enumerate(pos if len(pos) > 1 else pos * B):
+        if not 0 <= p < S:
+            assert not got[b].any()
 
 
 @pytest.mark.parametrize("B,heads,kv,dim,S,pos", DECODE)
@@ -221,7 +238,7 @@ def test_decode_with_vanishing_and_steep_scores(sgq, scale):
 PREFIX = [
     (1, 1, 1, 128, 4, [0], 1, 1), (2, 2, 2, 64, 16, [3, 15], 33, 40), (8, 16, 16, 128, 32, [9], 200, 256), (3, 12, 4, 64, 20, [0, 19, -1], 65, 65),
     (5, 8, 1, 128, 40, [39, 1, 2, 3, 40], 513, 600), (9, 14, 2, 128, 12, [4], 31, 64), (33, 4, 4, 64, 5, [2], 130, 130), (2, 16, 1, 64, 8, [7, 0], 3001, 3001),
-    (2, 4, 2, 128, 50, [49, 12], 0, 8), (2, 4, 2, 128, 50, [49, 12], -3, 8), (2, 4, 2, 128, 50, [49, 12], 99, 8), (70, 8, 2, 128, 6, [5], 90, 90)]
+    (2, 4, 2, 128, 50, [49, 12], 0, 8), (2, 4, 2, 128, 50, [49, 12], -3, 8), (2, 4, 2, 128, 50, [49, 12], 99, 8), (3, 8, 8, 128, 7000, [6999, -1, 3], 700, 720), (70, 8, 2, 128, 6, [5], 90, 90)]
 
 
 @pytest.mark.parametrize("B,heads,kv,dim,S,pos,prefix_len,prefix_max", PREFIX)
@@ -384,7 +401,7 @@ def test_the_c_calls_reject_what_they_cannot_run(sgq):
     """On a device: refused before anything is launched, and the context stays usable."""
     c = sgq.CacheInt8(256, 256, 256, 256, 1, 1, 8, 96)
     one = C.c_void_p(256)
-    assert sgq.lib.sgqd_attn_decode_int8(one, 288, 1, one, one, 8, one, 0, C.byref(c), one, 96, None, 0, None) == 4
+    assert sgq.lib.sgqd_attn_decode_int8(one, 288, 1, one, one, 8, one, 0, C.byref(c), one, 96, None, 0, None, 0, None) == 4
     cache = sgq.KVCacheInt8.empty(1, 1, 8, 96, "cuda")
     cos, sin = (dev(t) for t in plain.tables(8, 96))
     with pytest.raises(sgq.SgqError):

@@ -63,7 +63,7 @@ def decode(sgq, c, prefix=False, p=None, qkv=ONE, stride=1024, heads=4, cos=ONE,
            planes=None, nb=0, ws=ONE, wb=1 << 30):
     if prefix:
         return sgq.lib.sgqd_attn_decode_prefix_int8(qkv, stride, heads, cos, sin, rows, pos, ps, c, p, length, out, os, planes, nb, ws, wb, None)
-    return sgq.lib.sgqd_attn_decode_int8(qkv, stride, heads, cos, sin, rows, pos, ps, c, out, os, planes, nb, None)
+    return sgq.lib.sgqd_attn_decode_int8(qkv, stride, heads, cos, sin, rows, pos, ps, c, out, os, planes, nb, ws, wb, None)
 
 
 @pytest.mark.parametrize("prefix", [False, True])
@@ -88,12 +88,26 @@ def test_prefix_arguments(sgq):
     good = cache(sgq, batch=1, max_seq=32)
     assert decode(sgq, c, True, good, rows=48, length=None) == 1
     assert decode(sgq, c, True, cache(sgq, batch=1, max_seq=32, k=None), rows=48) == 1
-    need = sgq.lib.sgqd_attn_decode_prefix_int8_workspace_bytes(2, 4, 2, 128, 32)
-    if need:
-        assert decode(sgq, c, True, good, rows=48, ws=None) == 5 and decode(sgq, c, True, good, rows=48, wb=need - 1) == 5
-        assert decode(sgq, c, True, good, rows=48, ws=C.c_void_p(272)) == 5
-    for bad in ((0, 4, 2, 128, 32), (2, 4, 3, 128, 32), (2, 4, 0, 128, 32), (2, 4, 2, 96, 32), (2, 4, 2, 128, 0), (-1, 4, 2, 128, 32), (2, -4, 2, 128, 32)):
-        assert sgq.lib.sgqd_attn_decode_prefix_int8_workspace_bytes(*bad) == 0, bad
+    need = sgq.lib.sgqd_attn_decode_prefix_int8_workspace_bytes(2, 4, 2, 128, 16, 32)
+    assert need > 0
+    assert decode(sgq, c, True, good, rows=48, ws=None) == 5 and decode(sgq, c, True, good, rows=48, wb=need - 1) == 5
+    assert decode(sgq, c, True, good, rows=48, ws=C.c_void_p(272)) == 5
+
+
+def test_workspace_queries(sgq):
+    own, prefix = sgq.lib.sgqd_attn_decode_int8_workspace_bytes, sgq.lib.sgqd_attn_decode_prefix_int8_workspace_bytes
+    for bad in ((0, 4, 2, 128, 32), (2, 4, 3, 128, 32), (2, 4, 0, 128, 32), (2, 4, 2, 96, 32), (2, 4, 2, 128, 0), (-1, 4, 2, 128, 32), (2, -4, 2, 128, 32),
+                (2, 2 ** 20, 2, 128, 32), (2, 4, 2, 128, 2 ** 30 + 1), (2 ** 31, 4, 2, 128, 32)):
+        assert own(*bad) == 0 and prefix(*bad, 64) == 0, bad
+    assert prefix(2, 4, 2, 128, 32, 0) == 0 and prefix(2, 4, 2, 128, 32, -1) == 0 and prefix(2, 4, 2, 128, 32, 2 ** 30 + 1) == 0
+    assert own(1, 16, 16, 128, 640) == 0                                   # a short cache: joined inside a cluster of CTAs
+    assert own(32, 32, 8, 128, 8192) == 0                                  # and so are those of many sequences
+    need = own(2, 32, 8, 128, 65536)                                       # few long ones: partial results in the workspace
+    assert need > 0 and prefix(2, 32, 8, 128, 65536, 1024) > need
+    long = cache(sgq, batch=2, kv=8, max_seq=65536)
+    args = dict(stride=6144, heads=32, os=4096, rows=65536)
+    assert decode(sgq, long, ws=None, **args) == 5 and decode(sgq, long, wb=need - 1, **args) == 5 and decode(sgq, long, ws=C.c_void_p(264), **args) == 5
+    assert decode(sgq, cache(sgq, max_seq=2 ** 30 + 1), rows=2 ** 31) == 2
 
 
 # ---- the Python calls -----------------------------------------------------------------------------------------------
