@@ -16,6 +16,7 @@ cudaError_t read_status_gemm(uint32_t* v, bool clear);
 cudaError_t read_status_peer(uint32_t* v, bool clear);
 cudaError_t read_status_gemv_i8(uint32_t* v, bool clear);
 cudaError_t read_status_kn(uint32_t* v, bool clear);
+cudaError_t read_status_kv(uint32_t* v, bool clear);
 
 namespace {
 thread_local char g_error[512] = "";
@@ -257,7 +258,7 @@ unsigned int sgq_set_peer_wait_budget(unsigned int polls) {
 }
 
 int sgq_device_status(unsigned int* word, int clear) {
-    cudaError_t (*const readers[])(uint32_t*, bool) = {read_status_gemv, read_status_gemm, read_status_peer, read_status_gemv_i8, read_status_kn};
+    cudaError_t (*const readers[])(uint32_t*, bool) = {read_status_gemv, read_status_gemm, read_status_peer, read_status_gemv_i8, read_status_kn, read_status_kv};
     uint32_t v = 0;
     for (auto read : readers) {
         uint32_t w = 0;

@@ -5,11 +5,7 @@
 // code = clamp(round_half_away(r * (127 / a))), every operation rounded to fp32 (NaN -> +127, an infinity makes the scale
 // infinite).  The rotation in front of it rounds every product and sum to fp32 (no contraction), so codes and scales are a
 // function of the inputs alone: the prompt's store, the decode step's append and a host restatement agree in every bit.
-#include "sgq_common.cuh"
-#include "gemv_prepare.cuh"
-#include "sm100_ptx.cuh"
-
-#include "../../include/sgq_decoder.h"
+#include "kv_int8.cuh"
 
 #include <algorithm>
 #include <cooperative_groups.h>
@@ -21,13 +17,6 @@ namespace {
 
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxPositions = 1ll << 30;       // of the attention: positions and strides between tiles in 32 bits
-
-// (x1, x2) of a rotary pair, every operation rounded (src/ops.cpp:1737-1738)
-__device__ __forceinline__ void rotate_pair(float& x1, float& x2, float c, float s) {
-    const float a = __fsub_rn(__fmul_rn(x1, c), __fmul_rn(x2, s));
-    x2 = __fadd_rn(__fmul_rn(x2, c), __fmul_rn(x1, s));
-    x1 = a;
-}
 
 __device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
 
@@ -144,14 +133,6 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t
 // Scores and outputs leave the integer domain once per tile or step (sums of at most 128 products, below 2^21.1), scaled
 // and added in fp32 with the running reference and sum of the softmax.  A lane holds the scores of positions 4g .. 4g+3 and
 // the values [HD/8 g, HD/8 (g+1)) of the outputs of queries t and t + 4.
-struct CacheView {
-    int8_t* kc;
-    float* ks;
-    int8_t* vc;
-    float* vs;
-    int64_t max_seq;
-};
-
 // D = A(16x32, s8) * B(32x8, s8), and D += A * B
 __device__ __forceinline__ void mma_first(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
@@ -163,21 +144,6 @@ __device__ __forceinline__ void mma_next(int (&d)[4], uint32_t a0, uint32_t a1, 
         : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// The exact sum whose digit sums (2: highest; each below 2^21.1) these are, as fp32.  256 d2 + d1 fits an int32.
-__device__ __forceinline__ float join_digits(int d2, int d1, int d0) {
-    return fmaf(static_cast<float>(d2 * 256 + d1), 256.0f, static_cast<float>(d0));
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ float exp2_approx(float x) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-
 constexpr int kTile = 32;              // positions per step of a warp
 
 // ---- half tiles in shared memory: the 32 rows of keys or of values and their scales, fetched by cp.async -------------------
@@ -265,7 +231,7 @@ struct WarpAttention {
             for (int j = 0; j < VB; ++j) o[s][j] = 0.f;
         }
     }
-    // the digit planes and units of NQ queries, written by query_digits below
+    // the digit planes and units of NQ queries, written by query_planes below
     __device__ __forceinline__ void load_queries(const uint8_t* planes, const float* units) {
         auto rd = [&](uint32_t (&w)[KW], int query, int digit, bool zero) {
             const uint8_t* p = planes + query * kQueryBytes + digit * HD + 16 * t;
@@ -376,18 +342,15 @@ struct WarpAttention {
             }
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
-            // weights that vanish against the reference contribute nothing; NaN and infinity pass
-            const float per = most < 1e-30f ? 0.f : __fdividef(kDigitRange, most);
-            unit[s] = most * (1.0f / kDigitRange);
+            // weights that vanish against the reference contribute nothing; NaN and infinity make the unit NaN
+            const float per = most < 1e-30f ? 0.f : __fdividef(kWeightRange, most);
+            unit[s] = fmaf(most, 1.0f / kWeightRange, most - most);
 #pragma unroll
             for (int j = 0; j < ST; ++j) {
                 uint32_t d[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) d[i] = digit_bytes(__float2int_rn(sc[j][s][i] * per));
-                const uint32_t x = __byte_perm(d[0], d[1], 0x5140), y = __byte_perm(d[2], d[3], 0x5140);
-                w0[j][s] = __byte_perm(x, y, 0x5410);
-                w1[j][s] = __byte_perm(x, y, 0x7632);
-                w2[j][s] = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
+                for (int i = 0; i < 4; ++i) d[i] = weight_digits(sc[j][s][i], per);
+                gather_digits(d, w0[j][s], w1[j][s], w2[j][s]);
             }
         }
         // B fragments: lane (column g, position quad t or t + 4) takes the digit words that lane (quad, query) holds
@@ -468,43 +431,10 @@ struct WarpAttention {
     }
 };
 
-// One warp rotates a row of HD values, VEC consecutive per lane: lane l < 16 holds the first ones of the pairs of lane l + 16.
+// Digit planes [3][HD] of a query for WarpAttention::load_queries
 template <int HD>
-__device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos_row, const float* sin_row, int lane) {
-    constexpr int VEC = HD / 32;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) {
-        const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
-        const float c = cos_row[(lane & 15) * VEC + j], s = sin_row[(lane & 15) * VEC + j];
-        float x1 = lane < 16 ? v[j] : other, x2 = lane < 16 ? other : v[j];
-        rotate_pair(x1, x2, c, s);
-        v[j] = lane < 16 ? x1 : x2;
-    }
-}
-
-// The rotated query as digit planes [3][HD] and its unit, which carries 1/sqrt(HD) and log2(e).  A NaN or an infinity in the
-// query makes the unit NaN or infinite and the digits zero: every score is NaN.
-template <int HD>
-__device__ __forceinline__ void query_digits(const float (&v)[HD / 32], uint8_t* planes, float* unit, int lane) {
-    constexpr int VEC = HD / 32;
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    const float most = __uint_as_float(top);
-    const bool fine = top < 0x7F800000u && most >= 1e-30f;
-    const float per = fine ? __fdiv_rn(kDigitRange, most) : 0.f;
-    uint32_t d[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) d[j] = fine ? digit_bytes(__float2int_rn(__fmul_rn(v[j], per))) : 0u;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        if constexpr (VEC == 4)
-            *reinterpret_cast<uint32_t*>(planes + j * HD + lane * 4) = gather_byte(d[0], d[1], d[2], d[3], j);
-        else
-            *reinterpret_cast<uint16_t*>(planes + j * HD + lane * 2) = static_cast<uint16_t>(__byte_perm(d[0], d[1], 0x0040 + 0x11 * j));
-    }
-    if (lane == 0) *unit = top >= 0x7F800000u ? CUDART_NAN_F : (fine ? __fmul_rn(__fdiv_rn(most, kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f);
+__device__ __forceinline__ void query_planes(const float (&v)[HD / 32], uint8_t* planes, float* unit, int lane) {
+    query_digits<HD>(v, [&](int j, int d) { return planes + j * HD + d; }, unit, lane);
 }
 
 // One warp quantizes a row: its lane's codes (HD / 32 bytes) and the scale.
@@ -528,45 +458,6 @@ struct HeldRow {
         else *static_cast<uint16_t*>(row) = static_cast<uint16_t>(codes);
     }
 };
-
-struct DecodeArgs {
-    const float* qkv;
-    int64_t qkv_stride;
-    int n_heads, n_kv, batch;
-    const float* cos_t;
-    const float* sin_t;
-    const int32_t* pos;
-    int64_t pos_stride;
-    CacheView own, first;              // first: the shared prefix (prefix_len != NULL)
-    const int32_t* prefix_len;
-    float* out;
-    int64_t out_stride;
-    int pmode, nmain, nlow;
-    uint8_t* planes;
-    float* part_ml;                    // partial results of the prefix: [kv head][row][split][2] and [...][HD]
-    float* part_o;
-    int parts;                         // splits of the prefix, 0: none
-    float* flat_ml;                    // partial results of attn_flat_int8_kernel: [slot][NQ][2] and [slot][NQ][HD]
-    float* flat_o;
-};
-
-__device__ __forceinline__ int64_t prefix_rows(const DecodeArgs& a) {
-    if (!a.prefix_len) return 0;
-    const int64_t p = *a.prefix_len;
-    return p < 0 ? 0 : (p > a.first.max_seq ? a.first.max_seq : p);
-}
-
-// Joins partial results (maximum, sum, value) of one output value
-struct Joined {
-    float M, L, A;
-};
-__device__ __forceinline__ void join_part(Joined& j, float m, float l, float a) {
-    const float mn = fmaxf(j.M, m);
-    const float x = j.M == mn ? 1.0f : exp2_approx(j.M - mn), y = m == mn ? 1.0f : exp2_approx(m - mn);
-    j.L = fmaf(j.L, x, l * y);
-    j.A = fmaf(j.A, x, a * y);
-    j.M = mn;
-}
 
 // The rows a new token brings to a kv head, held by one warp.
 template <int HD>
@@ -696,7 +587,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
 #pragma unroll
     for (int i = 0; i < QPW; ++i) {
         rotate_row<HD>(qv[i], cos_row, sin_row, lane);
-        query_digits<HD>(qv[i], sm_q + (warp + i * W) * Attn::kQueryBytes, sm_unit + warp + i * W, lane);
+        query_planes<HD>(qv[i], sm_q + (warp + i * W) * Attn::kQueryBytes, sm_unit + warp + i * W, lane);
     }
     // The warp that takes the last tile stores the new token's rows (in one query block of the group).
     const bool owner = n > 0 && (n - 1) / STEP % (S * W) == split * W + warp;
@@ -785,7 +676,6 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
 // each unit it touches.  How many steps a unit has follows from `pos` alone, so every warp (and the kernel that joins the
 // results) finds its place by itself: nothing is handed out at run time and the result does not depend on timing.
 // The partial result of warp w for unit u goes to slot w + u: from one part of the row to the next w or u grows.
-constexpr int kSms = 148;                     // what the plans count on, whatever the device has
 constexpr int kFlatWarpsPerSm = 8, kFlatWarps = kSms * kFlatWarpsPerSm;
 template <int HD, int NQ>
 struct FlatShape {
@@ -907,7 +797,7 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
 #pragma unroll
                 for (int q = 0; q < NQ; ++q) {
                     rotate_row<HD>(qv[q], a.cos_t + turn, a.sin_t + turn, lane);
-                    query_digits<HD>(qv[q], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
+                    query_planes<HD>(qv[q], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
                 }
                 if (use.s + left >= use.T) {                               // the run holds the unit's last step
                     fresh.make(a, use.b, hk, a.cos_t + turn, a.sin_t + turn, lane);
@@ -1031,7 +921,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
-    static constexpr int ST = (QW == 1 ? 2 : 4) * (128 / HD) > 4 ? 4 : (QW == 1 ? 2 : 4) * (128 / HD);
+    static constexpr int ST = HD == 128 ? 2 : 4;
     static constexpr int kGroup = ST * Half<HD>::kBytes, kRing = KW * kGroups * kGroup;
     static constexpr int kOuts = kWarps * NQ * HD * 4;
     static constexpr int kQ = kRing > kOuts ? kRing : kOuts;
@@ -1094,7 +984,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const Dec
 #pragma unroll
     for (int i = 0; i < QW; ++i) {
         const int q = warp + i * kWarps;
-        query_digits<HD>(v[i], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
+        query_planes<HD>(v[i], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
     }
     __syncthreads();
     Attn w;
@@ -1158,19 +1048,20 @@ CacheView view(const sgqd_cache_int8* c) { return CacheView{c->k_codes, c->k_sca
 // Splits of a shared prefix and rows per block of its kernel: a function of the sizes alone, so that the workspace's size is one
 // too: the plans count 148 SMs, whatever the device has.
 struct PrefixPlan {
-    int qw, blocks, splits;
+    int qw;                              // warps side by side on 8 rows each, 0: the tcgen05 kernel
+    int blocks, splits;
     int64_t rows;                        // (kv head, query row) pairs
     size_t off_o, bytes;
 };
 PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t prefix_max) {
     PrefixPlan p = {};
     const int64_t R = batch * (n_heads / n_kv);
-    p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : (R <= 32 ? 4 : 8));
-    p.blocks = static_cast<int>(ceil_div(R, 8 * p.qw));
-    const int64_t most = ceil_div(prefix_max, kTile * (kWarps / p.qw));              // a tile for every group of warps
-    int64_t s = kSms / (n_kv * p.blocks);
-    s = s < 1 ? 1 : (s > most ? most : s);
-    p.splits = static_cast<int>(s > 65535 ? 65535 : s);
+    p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : 0);
+    const int64_t per_block = p.qw ? 8 * p.qw : kPrefixTcRows;
+    p.blocks = static_cast<int>(ceil_div(R, per_block));
+    const int64_t most = ceil_div(prefix_max, p.qw ? kTile * (kWarps / p.qw) : kPrefixTcTile);        // a tile for every group of warps
+    const int64_t s = std::min(kSms / (n_kv * p.blocks), most);
+    p.splits = static_cast<int>(std::min<int64_t>(std::max<int64_t>(s, 1), 65535));
     p.rows = n_kv * R;
     p.off_o = (static_cast<size_t>(p.rows) * p.splits * 8 + 255) / 256 * 256;
     p.bytes = p.off_o + static_cast<size_t>(p.rows) * p.splits * head_dim * 4;
@@ -1188,12 +1079,8 @@ int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
 }
 template <int HD>
 int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
-    switch (plan.qw) {
-        case 1: return launch_prefix<HD, 1>(a, plan, s);
-        case 2: return launch_prefix<HD, 2>(a, plan, s);
-        case 4: return launch_prefix<HD, 4>(a, plan, s);
-        default: return launch_prefix<HD, 8>(a, plan, s);
-    }
+    if (plan.qw == 0) return launch_prefix_tc(a, HD, plan.splits, plan.blocks, s);
+    return plan.qw == 1 ? launch_prefix<HD, 1>(a, plan, s) : launch_prefix<HD, 2>(a, plan, s);
 }
 
 // Which kernel reads the sequences' own rows.  `flat`: few units over long caches, where clusters cannot fill the device (one
