@@ -216,7 +216,7 @@ struct WarpAttention {
     static constexpr int kQueryBytes = 3 * HD; // digit planes of one query: [digit][HD]
     static constexpr float kAhead = 6.0f;
 
-    uint32_t bq[NT][KW];
+    const uint8_t* planes;                     // the queries' digits, in shared memory
     float qu[NS], m[NS], l[NS], o[NS][VB];
     int g, t;
 
@@ -232,7 +232,14 @@ struct WarpAttention {
         }
     }
     // the digit planes and units of NQ queries, written by query_planes below
-    __device__ __forceinline__ void load_queries(const uint8_t* planes, const float* units) {
+    __device__ __forceinline__ void use_queries(const uint8_t* digits, const float* units) {
+        planes = digits;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qu[s] = units[4 * s + t];
+    }
+    // B fragments of the digits: 16 to 24 registers that are read again for every step rather than kept through the products
+    // behind it (kept, the kernels do not fit three CTAs per SM)
+    __device__ __forceinline__ void load_queries(uint32_t (&bq)[NT][KW]) const {
         auto rd = [&](uint32_t (&w)[KW], int query, int digit, bool zero) {
             const uint8_t* p = planes + query * kQueryBytes + digit * HD + 16 * t;
 #pragma unroll
@@ -242,15 +249,12 @@ struct WarpAttention {
             }
         };
 #pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            rd(bq[s], 4 * s + (g >> 1), 2 - (g & 1), false);
-            qu[s] = units[4 * s + t];
-        }
+        for (int s = 0; s < NS; ++s) rd(bq[s], 4 * s + (g >> 1), 2 - (g & 1), false);
         if (NS == 2) rd(bq[NS], (g >> 1) + 4 * (g & 1), 0, false);
         else rd(bq[NS], g >> 1, 0, (g & 1) != 0);
     }
     // scores of a tile's keys: sc[s][i] of position 4g + i and query t + 4s, in base-2 units; positions from `n` on are masked
-    __device__ __forceinline__ void scores(float (&sc)[NS][4], const uint8_t* tile, int n) {
+    __device__ __forceinline__ void scores(float (&sc)[NS][4], const uint32_t (&bq)[NT][KW], const uint8_t* tile, int n) {
         uint32_t k[4][KW];
 #pragma unroll
         for (int i = 0; i < 4; ++i)
@@ -288,8 +292,10 @@ struct WarpAttention {
         }
     }
     __device__ __forceinline__ void scores_of(float (&sc)[ST][NS][4], const uint8_t* keys, const int (&n)[ST]) {
+        uint32_t bq[NT][KW];
+        load_queries(bq);
 #pragma unroll
-        for (int j = 0; j < ST; ++j) scores(sc[j], keys + j * Half<HD>::kBytes, n[j]);
+        for (int j = 0; j < ST; ++j) scores(sc[j], bq, keys + j * Half<HD>::kBytes, n[j]);
     }
     // A group of values, of which tile j has n[j] positions, with the scores: into the running sums and the outputs.  The
     // weights are taken against a reference that follows the maximum only when a score exceeds it by kAhead (weights up to
@@ -397,23 +403,24 @@ struct WarpAttention {
                     a[q][3] = __byte_perm(p1, p3, 0x7632);
                 }
 #pragma unroll
-                for (int pr = 0; pr < 2; ++pr)
+                for (int pr = 0; pr < 2; ++pr) {
+                    const int x = 2 * wd + pr;
 #pragma unroll
                     for (int n2 = 0; n2 < NT; ++n2) {
-                        if (j == 0) mma_first(acc[2 * wd + pr][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
-                        else mma_next(acc[2 * wd + pr][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
+                        if (j == 0) mma_first(acc[x][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
+                        else mma_next(acc[x][n2], a[0][2 * pr], a[0][2 * pr + 1], a[1][2 * pr], a[1][2 * pr + 1], bw[j][n2][0], bw[j][n2][1]);
                     }
+                    if (j < ST - 1) continue;
+#pragma unroll
+                    for (int s = 0; s < NS; ++s)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
+                            float& out = o[s][2 * x + e];
+                            out = fmaf(join_digits(acc[x][s][2 * e], acc[x][s][2 * e + 1], acc[x][NS][2 * e + s]), unit[s], out);
+                        }
+                }
             }
         }
-#pragma unroll
-        for (int x = 0; x < 2 * VW; ++x)
-#pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    float& out = o[s][2 * x + e];
-                    out = fmaf(join_digits(acc[x][s][2 * e], acc[x][s][2 * e + 1], acc[x][NS][2 * e + s]), unit[s], out);
-                }
     }
     // (reference, sum, value) of the first nq queries into to_ml[NQ][2], to_o[NQ][HD]
     __device__ __forceinline__ void store(float* to_ml, float* to_o, int nq = NQ) {
@@ -459,46 +466,64 @@ struct HeldRow {
     }
 };
 
-// The rows a new token brings to a kv head, held by one warp.
+// The rows a new token brings to a kv head: one warp makes them and keeps them in shared memory until it puts them into the
+// half tiles whose copies of the rows are older.
 template <int HD>
 struct NewRows {
-    HeldRow<HD> k, v;
-    __device__ __forceinline__ void make(const DecodeArgs& a, int b, int hk, const float* cos_row, const float* sin_row, int lane) {
+    static constexpr int kBytes = 2 * HD + 16;                             // codes of the key and of the value, their scales
+    static __device__ __forceinline__ void make(const DecodeArgs& a, int b, int hk, const float* cos_row, const float* sin_row, uint8_t* keep, int64_t row,
+                                                bool append, int lane) {
         constexpr int VEC = HD / 32;
-        const float* row = a.qkv + b * a.qkv_stride + lane * VEC;
+        const float* from = a.qkv + b * a.qkv_stride + static_cast<int64_t>(a.n_heads + hk) * HD + lane * VEC;
         float x[VEC], y[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
-            x[j] = row[static_cast<int64_t>(a.n_heads + hk) * HD + j];
-            y[j] = row[static_cast<int64_t>(a.n_heads + a.n_kv + hk) * HD + j];
+            x[j] = from[j];
+            y[j] = from[static_cast<int64_t>(a.n_kv) * HD + j];
         }
         rotate_row<HD>(x, cos_row, sin_row, lane);
+        HeldRow<HD> k, v;
         k.make(x);
         v.make(y);
+        k.put(keep + lane * VEC);
+        v.put(keep + HD + lane * VEC);
+        float* scales = reinterpret_cast<float*>(keep + 2 * HD);
+        if (lane == 0) { scales[0] = k.scale; scales[1] = v.scale; }
+        if (append) {
+            k.put(a.own.kc + row * HD + lane * VEC);
+            v.put(a.own.vc + row * HD + lane * VEC);
+            if (lane == 0) { a.own.ks[row] = k.scale; a.own.vs[row] = v.scale; }
+        }
+        __syncwarp();
     }
-    __device__ __forceinline__ void append(const DecodeArgs& a, int64_t row, int lane) const {
-        k.put(a.own.kc + row * HD + lane * (HD / 32));
-        v.put(a.own.vc + row * HD + lane * (HD / 32));
-        if (lane == 0) { a.own.ks[row] = k.scale; a.own.vs[row] = v.scale; }
-    }
-    // into row r of a half tile whose copy of the row is older
     template <bool KEYS>
-    __device__ __forceinline__ void bring_in(uint8_t* half, int r, int lane) const {
-        const HeldRow<HD>& h = KEYS ? k : v;
-        const int byte = lane * (HD / 32);
-        h.put(half + Half<HD>::template at<KEYS>(r, byte >> 4) + (byte & 15));
-        if (lane == 0) *reinterpret_cast<float*>(half + Half<HD>::kScales + 4 * r) = h.scale;
+    static __device__ __forceinline__ void bring_in(const uint8_t* keep, uint8_t* half, int r, int lane) {
+        if (lane < HD / 16)
+            *reinterpret_cast<uint4*>(half + Half<HD>::template at<KEYS>(r, lane)) = *reinterpret_cast<const uint4*>(keep + (KEYS ? 0 : HD) + lane * 16);
+        if (lane == 31) *reinterpret_cast<float*>(half + Half<HD>::kScales + 4 * r) = reinterpret_cast<const float*>(keep + 2 * HD)[KEYS ? 0 : 1];
         __syncwarp();
     }
 };
 
 // Finishes output value d of query head h of sequence b: the prefix's partial results, the division.
-template <int HD>
+template <int HD, bool PREFIX>
 __device__ __forceinline__ float finish(const DecodeArgs& a, Joined j, int b, int h, int d, bool live) {
-    const int G = a.n_heads / a.n_kv, hk = h / G;
-    if (live) {
+    if (PREFIX && live) {
+        const int G = a.n_heads / a.n_kv, hk = h / G;
         const int64_t p0 = (static_cast<int64_t>(hk) * a.batch * G + static_cast<int64_t>(b) * G + h - hk * G) * a.parts;
-        for (int p = 0; p < a.parts; ++p) join_part(j, a.part_ml[2 * (p0 + p)], a.part_ml[2 * (p0 + p) + 1], a.part_o[(p0 + p) * HD + d]);
+        constexpr int U = 6;                                           // loads on their way together
+        for (int p = 0; p < a.parts; p += U) {
+            float pm[U], pl[U], po[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const bool in = p + u < a.parts;
+                pm[u] = in ? a.part_ml[2 * (p0 + p + u)] : -CUDART_INF_F;
+                pl[u] = in ? a.part_ml[2 * (p0 + p + u) + 1] : 0.f;
+                po[u] = in ? a.part_o[(p0 + p + u) * HD + d] : 0.f;
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) join_part(j, pm[u], pl[u], po[u]);
+        }
     }
     const float o = j.L == 0.f ? 0.f : j.A / j.L;
     a.out[b * a.out_stride + static_cast<int64_t>(h) * HD + d] = o;
@@ -530,10 +555,13 @@ struct DecodeShape {
     static constexpr int kQ = kRing > kOuts ? kRing : kOuts;              // the warps' outputs take the ring's place at the end
     static constexpr int kPart = kQ + NQ * 3 * HD;
     static constexpr int kSmall = kPart + kRecv * HD * 4;                 // units [NQ], received [kRecv][2], ml [warps][NQ][2]
-    static constexpr int kBytes = kSmall + (NQ + 2 * kRecv + 2 * kDecodeWarps * NQ) * 4;
+    static constexpr int kNew = (kSmall + (NQ + 2 * kRecv + 2 * kDecodeWarps * NQ) * 4 + 15) / 16 * 16;
+    static constexpr int kBytes = kNew + NewRows<HD>::kBytes;
 };
-template <int HD, int NQ>
-__global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(const DecodeArgs a) {
+// PER_SM: CTAs that an SM has to hold.  With three the kernel keeps within 168 registers, where the compiler spills a few that it
+// needs at the end; with 2 it uses 175.
+template <int HD, int NQ, bool PREFIX, int PER_SM>
+__global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_kernel(const DecodeArgs a) {
     namespace cg = cooperative_groups;
     using Shape = DecodeShape<HD, NQ>;
     constexpr int VEC = HD / 32, W = kDecodeWarps, ST = Shape::ST, STEP = Shape::kStep, GROUP = Shape::kGroup;
@@ -551,25 +579,27 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
     pdl_launch_dependents();
     // Behind a prefix kernel only its partial results have to be waited for: that kernel lets this one start when
     // everything older than the two is complete.
-    if (a.parts == 0) pdl_wait();
+    if (!PREFIX) pdl_wait();
     if (S > 1) cluster_arrive();                                           // every CTA is there when it comes to storing into it
     const int b = blockIdx.x / a.n_kv, hk = blockIdx.x - b * a.n_kv, G = a.n_heads / a.n_kv;
     const int q0 = blockIdx.y * NQ, nq = min(NQ, G - q0);             // this block's queries of the group
     const int split = blockIdx.z;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int64_t base = (static_cast<int64_t>(b) * a.n_kv + hk) * a.own.max_seq;
-    const int8_t* kc = a.own.kc + base * HD;
-    const int8_t* vc = a.own.vc + base * HD;
-    const float* ks = a.own.ks + base;
-    const float* vs = a.own.vs + base;
     uint8_t* ring = sm + warp * kGroups * GROUP;
     const uint32_t ring_u = smem_u32(ring);
     const int first = (split * W + warp) * STEP, stride = S * W * STEP, rows = static_cast<int>(a.own.max_seq);
+    auto keys = [&](int to, int t, int end) {                              // asks for the step's keys, or values, at position t
+        request_group<HD, 32, ST, true>(ring_u + to * GROUP, a.own.kc + base * HD, a.own.ks + base, t, kTile, end, lane);
+        cp_async_commit();
+    };
+    auto values = [&](int to, int t, int end) {
+        request_group<HD, 32, ST, false>(ring_u + to * GROUP, a.own.vc + base * HD, a.own.vs + base, t, kTile, end, lane);
+        cp_async_commit();
+    };
     // The first tile is asked for before the position is known: its rows lie inside the cache in any case.
-    request_group<HD, 32, ST, true>(ring_u, kc, ks, first, kTile, rows, lane);
-    cp_async_commit();
-    request_group<HD, 32, ST, false>(ring_u + GROUP, vc, vs, first, kTile, rows, lane);
-    cp_async_commit();
+    keys(0, first, rows);
+    values(1, first, rows);
     const float* row = a.qkv + b * a.qkv_stride + static_cast<int64_t>(hk * G + q0) * HD + lane * VEC;
     float qv[QPW][VEC];
 #pragma unroll
@@ -578,12 +608,11 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
         for (int j = 0; j < VEC; ++j) qv[i][j] = warp + i * W < nq ? row[(warp + i * W) * HD + j] : 0.f;
     const int64_t pos = a.pos[b * a.pos_stride];
     const bool live = pos >= 0 && pos < a.own.max_seq;
-    const int64_t P = prefix_rows(a);
+    const int64_t P = PREFIX ? prefix_rows(a) : 0;
     const int n = live ? static_cast<int>(pos) + 1 : 0;
     const float* cos_row = a.cos_t + (live ? P + pos : 0) * (HD / 2);
     const float* sin_row = a.sin_t + (live ? P + pos : 0) * (HD / 2);
-    request_group<HD, 32, ST, true>(ring_u + 2 * GROUP, kc, ks, first + stride, kTile, n, lane);
-    cp_async_commit();
+    keys(2, first + stride, n);
 #pragma unroll
     for (int i = 0; i < QPW; ++i) {
         rotate_row<HD>(qv[i], cos_row, sin_row, lane);
@@ -591,15 +620,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
     }
     // The warp that takes the last tile stores the new token's rows (in one query block of the group).
     const bool owner = n > 0 && (n - 1) / STEP % (S * W) == split * W + warp;
-    NewRows<HD> fresh = {};
-    if (owner) {
-        fresh.make(a, b, hk, cos_row, sin_row, lane);
-        if (blockIdx.y == 0) fresh.append(a, base + pos, lane);
-    }
+    uint8_t* fresh = sm + Shape::kNew;
+    if (owner) NewRows<HD>::make(a, b, hk, cos_row, sin_row, fresh, base + pos, blockIdx.y == 0, lane);
     __syncthreads();
     Attn w;
     w.init(lane);
-    w.load_queries(sm_q, sm_unit);
+    w.use_queries(sm_q, sm_unit);
     int slot = 0;
     for (int t = first; t < n; t += stride) {
         int left[ST];
@@ -611,20 +637,18 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
         cp_async_wait<kGroups - 1>();
         __syncwarp();                                                      // the keys are there
         uint8_t* group = ring + slot * GROUP;
-        if (last) fresh.template bring_in<true>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+        if (last) NewRows<HD>::template bring_in<true>(fresh, group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
         w.scores_of(sc, group, left);
         __syncwarp();                                                      // everyone is through with them
-        request_group<HD, 32, ST, false>(ring_u + slot * GROUP, vc, vs, t + stride, kTile, n, lane);
-        cp_async_commit();
+        values(slot, t + stride, n);
         slot = next_slot(slot);
         cp_async_wait<kGroups - 1>();
         __syncwarp();
         group = ring + slot * GROUP;
-        if (last) fresh.template bring_in<false>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+        if (last) NewRows<HD>::template bring_in<false>(fresh, group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
         w.accumulate(sc, group, left);
         __syncwarp();
-        request_group<HD, 32, ST, true>(ring_u + slot * GROUP, kc, ks, t + 2 * stride, kTile, n, lane);
-        cp_async_commit();
+        keys(slot, t + 2 * stride, n);
         slot = next_slot(slot);
     }
     cp_async_wait<0>();
@@ -645,7 +669,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
             ml[1] = j.L;
         }
     }
-    if (a.parts != 0) pdl_wait();
+    if (PREFIX) pdl_wait();
     if (S > 1) {
         cluster_arrive();
         cluster_wait();
@@ -661,7 +685,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, 3) attn_decode_int8_kernel(
                 const int at = q / S * S + r;
                 join_part(j, sm_part_ml[2 * at], sm_part_ml[2 * at + 1], sm_part[at * HD + d]);
             }
-            sm_o[d] = finish<HD>(a, j, b, h, d, live);
+            sm_o[d] = finish<HD, PREFIX>(a, j, b, h, d, live);
         }
         if (a.planes != nullptr) {
             __syncthreads();
@@ -682,7 +706,8 @@ struct FlatShape {
     static constexpr int ST = HD == 128 ? 2 : 4, kStep = ST * kTile, kGroup = ST * Half<HD>::kBytes;
     static constexpr int kQ = kFlatWarpsPerSm * kGroups * kGroup;         // digits [W][NQ][3][HD]
     static constexpr int kSmall = kQ + kFlatWarpsPerSm * NQ * 3 * HD;     // units [W][NQ]
-    static constexpr int kBytes = kSmall + kFlatWarpsPerSm * NQ * 4;
+    static constexpr int kNew = kSmall + kFlatWarpsPerSm * NQ * 4;        // new rows [W]
+    static constexpr int kBytes = kNew + kFlatWarpsPerSm * NewRows<HD>::kBytes;
 };
 // How the row of steps is dealt out.  Every warp works it out, from 32 sequences at a time.
 struct FlatPlan {
@@ -704,14 +729,14 @@ struct FlatPlan {
         return __reduce_add_sync(0xffffffffu, front);
     }
 };
-template <int HD, int NQ>
+template <int HD, int NQ, bool PREFIX>
 __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(const DecodeArgs a, int blocks) {
     using Shape = FlatShape<HD, NQ>;
     constexpr int ST = Shape::ST, VEC = HD / 32, STEP = Shape::kStep;
     using Attn = WarpAttention<HD, NQ, ST>;
     extern __shared__ __align__(128) uint8_t sm[];
     pdl_launch_dependents();
-    if (a.parts == 0) pdl_wait();                                          // else at the end: see attn_decode_int8_kernel
+    if (!PREFIX) pdl_wait();                                          // else at the end: see attn_decode_int8_kernel
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.n_heads / a.n_kv, units_per_seq = a.n_kv * blocks;
     const int gw = blockIdx.x * kFlatWarpsPerSm + warp;
     uint8_t* ring = sm + warp * kGroups * Shape::kGroup;
@@ -780,14 +805,14 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
         request(false);
         request(true);
         Attn w;
-        NewRows<HD> fresh = {};
+        uint8_t* fresh = sm + Shape::kNew + warp * NewRows<HD>::kBytes;
         bool begin = true;
         int slot = 0;
         for (; left > 0; --left) {
             const int hk = use.j / blocks, qb = use.j - hk * blocks, q0 = qb * NQ, nq = min(NQ, G - q0);
             const bool end = use.s + 1 == use.T;                           // of the unit
             if (begin) {
-                const int64_t turn = (prefix_rows(a) + use.n - 1) * (HD / 2);
+                const int64_t turn = ((PREFIX ? prefix_rows(a) : 0) + use.n - 1) * (HD / 2);
                 const float* row = a.qkv + use.b * a.qkv_stride + static_cast<int64_t>(hk * G + q0) * HD + lane * VEC;
                 float qv[NQ][VEC];
 #pragma unroll
@@ -799,14 +824,12 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
                     rotate_row<HD>(qv[q], a.cos_t + turn, a.sin_t + turn, lane);
                     query_planes<HD>(qv[q], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
                 }
-                if (use.s + left >= use.T) {                               // the run holds the unit's last step
-                    fresh.make(a, use.b, hk, a.cos_t + turn, a.sin_t + turn, lane);
-                    if (qb == 0) fresh.append(a, (static_cast<int64_t>(use.b) * a.n_kv + hk) * a.own.max_seq + use.n - 1, lane);
-                }
+                if (use.s + left >= use.T)                                 // the run holds the unit's last step
+                    NewRows<HD>::make(a, use.b, hk, a.cos_t + turn, a.sin_t + turn, fresh,
+                                      (static_cast<int64_t>(use.b) * a.n_kv + hk) * a.own.max_seq + use.n - 1, qb == 0, lane);
                 __syncwarp();
                 w.init(lane);
-                w.load_queries(sm_q, sm_unit);
-                __syncwarp();                                              // everyone has read the digits
+                w.use_queries(sm_q, sm_unit);
                 begin = false;
             }
             int in[ST];
@@ -817,7 +840,7 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
             cp_async_wait<kGroups - 1>();
             __syncwarp();                                                  // the keys are there
             uint8_t* group = ring + slot * Shape::kGroup;
-            if (end) fresh.template bring_in<true>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+            if (end) NewRows<HD>::template bring_in<true>(fresh, group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
             w.scores_of(sc, group, in);
             __syncwarp();                                                  // everyone is through with them
             request(false);
@@ -825,7 +848,7 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
             cp_async_wait<kGroups - 1>();
             __syncwarp();
             group = ring + slot * Shape::kGroup;
-            if (end) fresh.template bring_in<false>(group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
+            if (end) NewRows<HD>::template bring_in<false>(fresh, group + r / kTile * Half<HD>::kBytes, r % kTile, lane);
             w.accumulate(sc, group, in);
             __syncwarp();
             request(true);
@@ -839,13 +862,13 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
         }
     }
     cp_async_wait<0>();
-    if (a.parts != 0) pdl_wait();
+    if (PREFIX) pdl_wait();
 }
 
 // Joins the partial results of attn_flat_int8_kernel (and of a prefix).  WIDE: a block per (sequence, query head), whose warps take
 // the slots in turn; else a warp per (sequence, query head).  A lane holds HD / 32 values.  Where the slots are follows from
 // `pos`, which is older than the kernel in front: that is worked out before its results are waited for.
-template <int HD, int NQ, bool WIDE>
+template <int HD, int NQ, bool WIDE, bool PREFIX>
 __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const DecodeArgs a, int blocks) {
     constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, BY = WIDE ? kWarps : 1, U = 6;
     __shared__ float sm_ml[kWarps][2];
@@ -901,7 +924,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
             Joined t = {-CUDART_INF_F, 0.f, 0.f};
 #pragma unroll
             for (int u = 0; u < kWarps; ++u) join_part(t, sm_ml[u][0], sm_ml[u][1], sm_o[u][d]);
-            sm_o[0][d] = finish<HD>(a, t, b, h, d, T > 0);
+            sm_o[0][d] = finish<HD, PREFIX>(a, t, b, h, d, T > 0);
         }
         if (a.planes == nullptr) return;
         __syncthreads();
@@ -909,7 +932,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
     } else {
         if (!there) return;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = finish<HD>(a, Joined{m, l, o[i]}, b, h, lane * VEC + i, T > 0);
+        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = finish<HD, PREFIX>(a, Joined{m, l, o[i]}, b, h, lane * VEC + i, T > 0);
         __syncwarp();
         if (a.planes != nullptr) prepare_head<HD>(a, &sm_o[warp][0], b, h, lane);
     }
@@ -989,7 +1012,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_prefix_int8_kernel(const Dec
     __syncthreads();
     Attn w;
     w.init(lane);
-    w.load_queries(sm_q + qg * NQ * Attn::kQueryBytes, sm_unit + qg * NQ);
+    w.use_queries(sm_q + qg * NQ * Attn::kQueryBytes, sm_unit + qg * NQ);
     int slot = 0;
     for (int t = first; t < t1; t += STRIDE) {
         int left[ST];
@@ -1105,37 +1128,25 @@ DecodePlan decode_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t hea
         p.off_o = (slots * p.nq * 8 + 255) / 256 * 256;
         p.bytes = p.off_o + slots * p.nq * head_dim * 4;
     }
-    // Splits: enough CTAs for sequences of unequal length to even out (about 1000, three of them per SM: batch 32 x 8 heads of up
-    // to 8192 positions 76 / 58 / 56 / 55 / 62 us with 1 / 2 / 3 / 4 / 8 splits), with two steps for each warp or, where the
-    // units do not fill the SMs, one (batch 8 x 16 heads, 576 positions: 9.0 / 12.7 us with 2 / 4; batch 5 x 4 heads of 64,
-    // up to 1500: 6.6 / 6.0 with 3 / 6).
+    // Splits: the least of waves x (what a CTA costs beside its steps, in steps: 3, and 1 for each CTA that shares the SM, + steps of a
+    // warp).  Measured (us): batch 8 x 16 heads, 576 positions 9.6 / 8.8 / 10.8 / 12.7 with 1 / 2 / 3 / 4 splits; batch 32 x 8
+    // heads, 512 positions 9 / 16 with 1 / 2, of up to 8192 76 / 58 / 56 / 55 / 62 with 1 / 2 / 3 / 4 / 8; batch 37 x 16, 2048
+    // positions 63 / 57 / 65 with 1 / 2 / 4.
     const int64_t steps = ceil_div(max_seq, (128 / head_dim) * kTile);
-    int64_t S = (1000 + units / 2) / units;
-    const int64_t two = steps / (2 * kDecodeWarps), fill = 2 * kSms / units, one = ceil_div(steps, kDecodeWarps);
-    S = std::min(std::min(S, one), std::max(two, fill));
-    p.splits = static_cast<int>(std::max<int64_t>(std::min<int64_t>(S, kMaxSplits), 1));
+    int64_t least = 0;
+    for (int S = 1; S <= kMaxSplits; ++S) {
+        const int64_t ctas = units * S, waves = ceil_div(ctas, 3 * kSms), shared = std::min<int64_t>(ceil_div(ctas, kSms), 3);
+        const int64_t cost = waves * (3 + shared + ceil_div(steps, kDecodeWarps * S));
+        if (S == 1 || cost < least) { least = cost; p.splits = S; }
+    }
     return p;
 }
 
-template <int HD, int NQ>
-int launch_decode(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
-    if (plan.flat) {
-        static SmemOptIn opt_in;
-        constexpr int bytes = FlatShape<HD, NQ>::kBytes;
-        SGQ_CUDA_TRY(opt_in.ensure(attn_flat_int8_kernel<HD, NQ>, bytes));
-        SGQ_CUDA_TRY(launch_kernel(attn_flat_int8_kernel<HD, NQ>, dim3(kSms), dim3(kFlatWarpsPerSm * 32), bytes, s, true, a, plan.blocks));
-        const int64_t heads = static_cast<int64_t>(a.batch) * a.n_heads;
-        // a head has about kFlatWarps / units slots: with more than a warp asks for at once, a block takes it
-        if (plan.units * 6 < kFlatWarps)
-            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, true>, dim3(static_cast<unsigned>(heads)), dim3(kWarps * 32), 0, s, true, a, plan.blocks));
-        else
-            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, false>, dim3(static_cast<unsigned>(ceil_div(heads, kWarps))), dim3(kWarps * 32), 0, s, true,
-                                       a, plan.blocks));
-        return SGQ_OK;
-    }
+template <int HD, int NQ, bool PREFIX, int PER_SM>
+int launch_clusters(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
     static SmemOptIn opt_in;
     constexpr int bytes = DecodeShape<HD, NQ>::kBytes;
-    SGQ_CUDA_TRY(opt_in.ensure(attn_decode_int8_kernel<HD, NQ>, bytes));
+    SGQ_CUDA_TRY(opt_in.ensure(attn_decode_int8_kernel<HD, NQ, PREFIX, PER_SM>, bytes));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(static_cast<unsigned>(a.batch * a.n_kv), static_cast<unsigned>(plan.blocks), static_cast<unsigned>(plan.splits));
     cfg.blockDim = dim3(kDecodeWarps * 32);
@@ -1150,8 +1161,37 @@ int launch_decode(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
     attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    SGQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_decode_int8_kernel<HD, NQ>, a));
+    SGQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, attn_decode_int8_kernel<HD, NQ, PREFIX, PER_SM>, a));
     return SGQ_OK;
+}
+template <int HD, int NQ, bool PREFIX>
+int launch_decode(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
+    if (plan.flat) {
+        static SmemOptIn opt_in;
+        constexpr int bytes = FlatShape<HD, NQ>::kBytes;
+        SGQ_CUDA_TRY(opt_in.ensure(attn_flat_int8_kernel<HD, NQ, PREFIX>, bytes));
+        SGQ_CUDA_TRY(launch_kernel(attn_flat_int8_kernel<HD, NQ, PREFIX>, dim3(kSms), dim3(kFlatWarpsPerSm * 32), bytes, s, true, a, plan.blocks));
+        const int64_t heads = static_cast<int64_t>(a.batch) * a.n_heads;
+        // a head has about kFlatWarps / units slots: with more than a warp asks for at once, a block takes it
+        if (plan.units * 6 < kFlatWarps)
+            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, true, PREFIX>, dim3(static_cast<unsigned>(heads)), dim3(kWarps * 32), 0, s, true, a, plan.blocks));
+        else
+            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, false, PREFIX>, dim3(static_cast<unsigned>(ceil_div(heads, kWarps))), dim3(kWarps * 32), 0, s, true,
+                                       a, plan.blocks));
+        return SGQ_OK;
+    }
+    // Where two per SM take the whole grid, the form that spills nothing (8 x 16 heads, 576 positions: 8.9 -> 8.2 us; 32 x 8 heads,
+    // 512 positions 11.4 -> 9.9); else three (32 x 8 heads, 8192 positions: 59 -> 57).
+    if constexpr ((HD == 128) == (NQ == 4)) {
+        if (plan.units * plan.splits <= 2 * kSms) return launch_clusters<HD, NQ, PREFIX, 2>(a, plan, s);
+    }
+    return launch_clusters<HD, NQ, PREFIX, 3>(a, plan, s);
+}
+
+template <bool PREFIX>
+int launch_decode(const DecodeArgs& a, int64_t head_dim, const DecodePlan& plan, cudaStream_t s) {
+    if (head_dim == 128) return plan.nq == 4 ? launch_decode<128, 4, PREFIX>(a, plan, s) : launch_decode<128, 8, PREFIX>(a, plan, s);
+    return plan.nq == 4 ? launch_decode<64, 4, PREFIX>(a, plan, s) : launch_decode<64, 8, PREFIX>(a, plan, s);
 }
 
 size_t decode_workspace(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t max_seq, int64_t prefix_max) {
@@ -1195,7 +1235,7 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
     const size_t need = decode_workspace(batch, n_heads, kv, hd, cache->max_seq, prefix ? prefix->max_seq : 0);
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
         return bad(SGQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
-    if (batch * n_heads > 0x7fffffff) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
+    if (batch * n_heads > 0x7fffff00) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
     if ((rc = check_device()) != SGQ_OK) return rc;
     DecodeArgs a = {};
     a.qkv = qkv; a.qkv_stride = qkv_stride; a.n_heads = static_cast<int>(n_heads); a.n_kv = static_cast<int>(kv); a.batch = static_cast<int>(batch);
@@ -1216,8 +1256,7 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
         rc = hd == 128 ? launch_prefix<128>(a, first, s) : launch_prefix<64>(a, first, s);
         if (rc != SGQ_OK) return rc;
     }
-    if (hd == 128) return plan.nq == 4 ? launch_decode<128, 4>(a, plan, s) : launch_decode<128, 8>(a, plan, s);
-    return plan.nq == 4 ? launch_decode<64, 4>(a, plan, s) : launch_decode<64, 8>(a, plan, s);
+    return prefix ? launch_decode<true>(a, hd, plan, s) : launch_decode<false>(a, hd, plan, s);
 }
 
 }  // namespace

@@ -97,18 +97,27 @@ __device__ __forceinline__ void join_part(Joined& j, float m, float l, float a) 
     j.M = mn;
 }
 
-// One warp rotates a row of HD values, VEC consecutive per lane: lane l < 16 holds the first ones of the pairs of lane l + 16.
+// One warp rotates a row of HD values, VEC consecutive per lane: lane l < 16 holds the first ones of the pairs of lane l + 16.  c, s:
+// the cosines and sines of pairs (lane & 15) VEC ..
 template <int HD>
-__device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos_row, const float* sin_row, int lane) {
-    constexpr int VEC = HD / 32;
+__device__ __forceinline__ void rotate_values(float (&v)[HD / 32], const float (&c)[HD / 32], const float (&s)[HD / 32], int lane) {
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) {
+    for (int j = 0; j < HD / 32; ++j) {
         const float other = __shfl_xor_sync(0xffffffffu, v[j], 16);
-        const float c = cos_row[(lane & 15) * VEC + j], s = sin_row[(lane & 15) * VEC + j];
         float x1 = lane < 16 ? v[j] : other, x2 = lane < 16 ? other : v[j];
-        rotate_pair(x1, x2, c, s);
+        rotate_pair(x1, x2, c[j], s[j]);
         v[j] = lane < 16 ? x1 : x2;
     }
+}
+template <int HD>
+__device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos_row, const float* sin_row, int lane) {
+    float c[HD / 32], s[HD / 32];
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) {
+        c[j] = cos_row[(lane & 15) * (HD / 32) + j];
+        s[j] = sin_row[(lane & 15) * (HD / 32) + j];
+    }
+    rotate_values<HD>(v, c, s, lane);
 }
 
 // The rotated query as digits (at(j, d): where digit j of value d goes) and its unit, which carries 1/sqrt(HD) and log2(e).  A
