@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <cooperative_groups.h>
+#include <math.h>
 #include <math_constants.h>
 
 namespace sgq {
@@ -505,30 +506,6 @@ struct NewRows {
     }
 };
 
-// Finishes output value d of query head h of sequence b: the prefix's partial results, the division.
-template <int HD, bool PREFIX>
-__device__ __forceinline__ float finish(const DecodeArgs& a, Joined j, int b, int h, int d, bool live) {
-    if (PREFIX && live) {
-        const int G = a.n_heads / a.n_kv, hk = h / G;
-        const int64_t p0 = (static_cast<int64_t>(hk) * a.batch * G + static_cast<int64_t>(b) * G + h - hk * G) * a.parts;
-        constexpr int U = 6;                                           // loads on their way together
-        for (int p = 0; p < a.parts; p += U) {
-            float pm[U], pl[U], po[U];
-#pragma unroll
-            for (int u = 0; u < U; ++u) {
-                const bool in = p + u < a.parts;
-                pm[u] = in ? a.part_ml[2 * (p0 + p + u)] : -CUDART_INF_F;
-                pl[u] = in ? a.part_ml[2 * (p0 + p + u) + 1] : 0.f;
-                po[u] = in ? a.part_o[(p0 + p + u) * HD + d] : 0.f;
-            }
-#pragma unroll
-            for (int u = 0; u < U; ++u) join_part(j, pm[u], pl[u], po[u]);
-        }
-    }
-    const float o = j.L == 0.f ? 0.f : j.A / j.L;
-    a.out[b * a.out_stride + static_cast<int64_t>(h) * HD + d] = o;
-    return o;
-}
 // One warp: a finished head as prepared activations of the [batch, n_heads * HD] matrix (a head is HD / 32 whole groups)
 template <int HD>
 __device__ __forceinline__ void prepare_head(const DecodeArgs& a, const float* head, int b, int h, int lane) {
@@ -539,6 +516,81 @@ __device__ __forceinline__ void prepare_head(const DecodeArgs& a, const float* h
     const PreparedParts pp = prepared_parts(a.planes, static_cast<size_t>(a.n_heads) * (HD / 32), a.nmain, a.nlow);
     convert_groups<kOrderNibble>(v, b, a.batch, static_cast<size_t>(h) * (HD / 32), a.pmode, a.nmain, a.nlow, 0.0625f, pp, in);
 }
+
+// One warp's share of a head: the partial result of HD / 32 values per lane.
+template <int HD>
+struct JoinedHead {
+    static constexpr int VEC = HD / 32;
+    float M, L, A[VEC];
+    __device__ __forceinline__ JoinedHead() : M(-HUGE_VALF), L(0.f) {
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) A[i] = 0.f;
+    }
+    // the partial results i < n of which `load` gives reference, sum and this lane's values; U of them are asked for together
+    template <int U, typename Load>
+    __device__ __forceinline__ void join(int n, Load load) {
+        for (int p = 0; p < n; p += U) {
+            float m[U], l[U], v[U][VEC];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                m[u] = -CUDART_INF_F;
+                l[u] = 0.f;
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) v[u][i] = 0.f;
+                if (p + u < n) load(p + u, m[u], l[u], v[u]);
+            }
+            float mn = M;
+#pragma unroll
+            for (int u = 0; u < U; ++u) mn = fmaxf(mn, m[u]);
+            const float x = M == mn ? 1.0f : exp2_approx(M - mn);
+            L *= x;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) A[i] *= x;
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const float y = m[u] == mn ? 1.0f : exp2_approx(m[u] - mn);
+                L = fmaf(l[u], y, L);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) A[i] = fmaf(v[u][i], y, A[i]);
+            }
+            M = mn;
+        }
+    }
+    static __device__ __forceinline__ void load(const float* from, float (&v)[VEC]) {
+        if constexpr (VEC == 4) {
+            const float4 x = *reinterpret_cast<const float4*>(from);
+            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+        } else {
+            const float2 x = *reinterpret_cast<const float2*>(from);
+            v[0] = x.x; v[1] = x.y;
+        }
+    }
+    // joins the prefix's partial results, divides, stores query head h of sequence b (`head`: HD floats of shared memory)
+    template <bool PREFIX>
+    __device__ __forceinline__ void finish(const DecodeArgs& a, int b, int h, bool live, float* head, int lane) {
+        if (PREFIX && live) {
+            const int G = a.n_heads / a.n_kv, hk = h / G;
+            const int64_t p0 = (static_cast<int64_t>(hk) * a.batch * G + static_cast<int64_t>(b) * G + h - hk * G) * a.parts;
+            join<6>(a.parts, [&](int p, float& m, float& l, float (&v)[VEC]) {
+                m = a.part_ml[2 * (p0 + p)];
+                l = a.part_ml[2 * (p0 + p) + 1];
+                load(a.part_o + (p0 + p) * HD + lane * VEC, v);
+            });
+        }
+        float* to = a.out + b * a.out_stride + static_cast<int64_t>(h) * HD + lane * VEC;
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const float o = L == 0.f ? 0.f : A[i] / L;
+            to[i] = o;
+            head[lane * VEC + i] = o;
+        }
+        if (a.planes != nullptr) {
+            __syncwarp();
+            prepare_head<HD>(a, head, b, h, lane);
+            __syncwarp();
+        }
+    }
+};
 
 constexpr int kWarps = 8;
 // Short caches.  grid (batch * kv heads, query blocks, S) in clusters of S along z: the W warps of the S CTAs of a cluster take
@@ -676,22 +728,14 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
     } else {
         __syncthreads();
     }
-    for (int q = split; q < nq; q += S) {
-        const int h = hk * G + q0 + q;
-        if (threadIdx.x < HD) {
-            const int d = threadIdx.x;
-            Joined j = {-CUDART_INF_F, 0.f, 0.f};
-            for (int r = 0; r < S; ++r) {
-                const int at = q / S * S + r;
-                join_part(j, sm_part_ml[2 * at], sm_part_ml[2 * at + 1], sm_part[at * HD + d]);
-            }
-            sm_o[d] = finish<HD, PREFIX>(a, j, b, h, d, live);
-        }
-        if (a.planes != nullptr) {
-            __syncthreads();
-            if (warp == 0) prepare_head<HD>(a, sm_o, b, h, lane);
-            __syncthreads();
-        }
+    for (int i = warp; split + i * S < nq; i += W) {                       // a warp finishes every W-th of this CTA's heads
+        JoinedHead<HD> j;
+        j.template join<4>(S, [&](int r, float& m, float& l, float (&v)[VEC]) {
+            m = sm_part_ml[2 * (i * S + r)];
+            l = sm_part_ml[2 * (i * S + r) + 1];
+            JoinedHead<HD>::load(sm_part + (i * S + r) * HD + lane * VEC, v);
+        });
+        j.template finish<PREFIX>(a, b, hk * G + q0 + split + i * S, live, sm_o + warp * HD, lane);
     }
 }
 
@@ -870,7 +914,7 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
 // `pos`, which is older than the kernel in front: that is worked out before its results are waited for.
 template <int HD, int NQ, bool WIDE, bool PREFIX>
 __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const DecodeArgs a, int blocks) {
-    constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, BY = WIDE ? kWarps : 1, U = 6;
+    constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, BY = WIDE ? kWarps : 1;
     __shared__ float sm_ml[kWarps][2];
     __shared__ __align__(16) float sm_o[kWarps][HD];
     pdl_launch_dependents();
@@ -883,59 +927,30 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
     const int front = plan.make(a, units_per_seq, b, STEP, lane) * units_per_seq, T = FlatPlan::steps(a, b, STEP);
     const int start = front + j * T, w0 = start / plan.per, w1 = T > 0 ? (start + T - 1) / plan.per : w0 - 1;
     const int64_t unit = static_cast<int64_t>(b) * units_per_seq + j;
-    float m = -CUDART_INF_F, l = 0.f, o[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) o[i] = 0.f;
+    JoinedHead<HD> t;
     pdl_wait();
-    for (int w = w0 + (WIDE ? warp : 0); w <= w1; w += U * BY) {
-        float pm[U], pl[U], po[U][VEC];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const bool in = w + u * BY <= w1;
-            const int64_t at = (unit + (in ? w + u * BY : w)) * NQ + g % NQ;
-            pm[u] = in ? a.flat_ml[2 * at] : -CUDART_INF_F;
-            pl[u] = in ? a.flat_ml[2 * at + 1] : 0.f;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) po[u][i] = in ? a.flat_o[at * HD + lane * VEC + i] : 0.f;
-        }
-        float mn = m;
-#pragma unroll
-        for (int u = 0; u < U; ++u) mn = fmaxf(mn, pm[u]);
-        const float x = m == mn ? 1.0f : exp2_approx(m - mn);
-        l *= x;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) o[i] *= x;
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const float y = pm[u] == mn ? 1.0f : exp2_approx(pm[u] - mn);
-            l = fmaf(pl[u], y, l);
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) o[i] = fmaf(po[u][i], y, o[i]);
-        }
-        m = mn;
-    }
+    const int w_first = w0 + (WIDE ? warp : 0);
+    t.template join<6>(w_first <= w1 ? (w1 - w_first) / BY + 1 : 0, [&](int p, float& m, float& l, float (&v)[VEC]) {
+        const int64_t at = (unit + w_first + p * BY) * NQ + g % NQ;
+        m = a.flat_ml[2 * at];
+        l = a.flat_ml[2 * at + 1];
+        JoinedHead<HD>::load(a.flat_o + at * HD + lane * VEC, v);
+    });
     if constexpr (WIDE) {
-        if (lane == 0) { sm_ml[warp][0] = m; sm_ml[warp][1] = l; }
+        if (lane == 0) { sm_ml[warp][0] = t.M; sm_ml[warp][1] = t.L; }
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = o[i];
+        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = t.A[i];
         __syncthreads();
-        if (threadIdx.x < HD) {
-            const int d = threadIdx.x;
-            Joined t = {-CUDART_INF_F, 0.f, 0.f};
-#pragma unroll
-            for (int u = 0; u < kWarps; ++u) join_part(t, sm_ml[u][0], sm_ml[u][1], sm_o[u][d]);
-            sm_o[0][d] = finish<HD, PREFIX>(a, t, b, h, d, T > 0);
-        }
-        if (a.planes == nullptr) return;
-        __syncthreads();
-        if (warp == 0) prepare_head<HD>(a, &sm_o[0][0], b, h, lane);
-    } else {
-        if (!there) return;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) sm_o[warp][lane * VEC + i] = finish<HD, PREFIX>(a, Joined{m, l, o[i]}, b, h, lane * VEC + i, T > 0);
+        if (warp != 0) return;
+        t = JoinedHead<HD>();
+        t.template join<4>(kWarps, [&](int u, float& m, float& l, float (&v)[VEC]) {
+            m = sm_ml[u][0];
+            l = sm_ml[u][1];
+            JoinedHead<HD>::load(&sm_o[u][lane * VEC], v);
+        });
         __syncwarp();
-        if (a.planes != nullptr) prepare_head<HD>(a, &sm_o[warp][0], b, h, lane);
     }
+    if (there) t.template finish<PREFIX>(a, b, h, T > 0, &sm_o[warp][0], lane);
 }
 
 // Partial attention of every sequence's queries to the shared prefix.  grid (kv heads, splits of the prefix, blocks of 8 QW rows),

@@ -49,6 +49,18 @@ __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 
+template <int N>
+__device__ __forceinline__ void load_values_of(const float* from, float (&v)[N]) {
+    static_assert(N == 2 || N == 4, "head sizes of 64 and 128");
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(from);
+        v[0] = x.x; v[1] = x.y;
+    }
+}
+
 // grid (kv heads, splits of the prefix, blocks of 128 rows)
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const DecodeArgs a) {
@@ -162,11 +174,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             for (int i = 0; i < 4; ++i) {
                 const int at = __shfl_sync(0xffffffffu, turn, i0 + i);
                 const int64_t from = static_cast<int64_t>(max(at, 0)) * (HD / 2) + (lane & 15) * VEC;
+                load_values_of(a.cos_t + from, co[i]);
+                load_values_of(a.sin_t + from, si[i]);
+                load_values_of(rows + (i0 + i) * HD + lane * VEC, q[i]);
+                if (at < 0) {
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) {
-                    co[i][j] = a.cos_t[from + j];
-                    si[i][j] = a.sin_t[from + j];
-                    q[i][j] = at < 0 ? 0.f : rows[(i0 + i) * HD + lane * VEC + j];
+                    for (int j = 0; j < VEC; ++j) q[i][j] = 0.f;
                 }
             }
 #pragma unroll
