@@ -19,13 +19,33 @@ namespace {
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxPositions = 1ll << 30;       // of the attention: positions and strides between tiles in 32 bits
 
-__device__ __forceinline__ float4 ld4(const float* p) { return *reinterpret_cast<const float4*>(p); }
+// N = 4 or 8 consecutive floats, aligned to their own size
+template <int N>
+__device__ __forceinline__ void load_floats(float (&v)[N], const float* p) {
+    if constexpr (N == 8)
+        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(p)
+                     : "memory");
+    else {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
+    if constexpr (N == 8)
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+                     "f"(v[6]), "f"(v[7])
+                     : "memory");
+    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
 
 // ---- store ------------------------------------------------------------------------------------------------------------
-// One group of LPR lanes per row (a head of q, k or v of one token); a lane owns the values 4l .. 4l+3 of the first half of the
-// row and of the second half, so that a rotary pair sits in one lane and only the absmax crosses lanes.
-constexpr int kStoreThreads = 256;
-template <int LPR>
+// One group of LPR lanes per row (a head of q, k or v of one token); a lane owns VEC values of the first half of the row and the
+// same VEC of the second half, so that a rotary pair sits in one lane and only the absmax crosses lanes.  grid (tokens, row blocks).
+constexpr int kStoreThreads = 256;                   // at most; the rows of a token are dealt out evenly to its blocks
+template <int LPR, int VEC>
 __global__ void __launch_bounds__(kStoreThreads) rope_kv_store_int8_kernel(const float* qkv, int64_t qkv_stride, int t_new, int n_heads, int n_kv,
                                                                            int head_dim, const float* __restrict__ cos_t,
                                                                            const float* __restrict__ sin_t, int64_t table_rows,
@@ -37,82 +57,105 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_store_int8_kernel(const
     pdl_launch_dependents();
     pdl_wait();
     const int64_t m = blockIdx.x;
-    const int b = static_cast<int>(m / t_new), i = static_cast<int>(m - static_cast<int64_t>(b) * t_new);
-    const int r = blockIdx.y * (kStoreThreads / LPR) + threadIdx.x / LPR;      // row of the token: q heads, k heads, v heads
+    const int b = static_cast<int>(blockIdx.x / static_cast<unsigned>(t_new)), i = static_cast<int>(m - static_cast<int64_t>(b) * t_new);
+    const int r = blockIdx.y * (blockDim.x / LPR) + threadIdx.x / LPR;          // row of the token: q heads, k heads, v heads
     const int l = threadIdx.x % LPR;
     const int half = head_dim >> 1;
-    const bool in = r < n_heads + 2 * n_kv && 4 * l < half;
-    const float* row = qkv + m * qkv_stride + static_cast<int64_t>(r) * head_dim + 4 * l;
-    float4 a = make_float4(0.f, 0.f, 0.f, 0.f), c = a;
-    if (in) { a = ld4(row); c = ld4(row + half); }
+    const bool in = r < n_heads + 2 * n_kv && VEC * l < half;
+    const float* row = qkv + m * qkv_stride + static_cast<int64_t>(r) * head_dim + VEC * l;
     const int64_t pos = static_cast<int64_t>(pos_p[b * pos_stride]) + i;
     const int64_t turn = pos + (rope_offset ? *rope_offset : 0);
     // a token behind the sequence's own count, outside the cache or outside the tables leaves everything as it was
     if (pos < 0 || pos >= max_seq || turn < 0 || turn >= table_rows || (n_new && i >= n_new[b])) return;         // uniform over the block
-    if (r < n_heads + n_kv && in) {
-        const int64_t at = turn * half + 4 * l;
-        const float4 co = ld4(cos_t + at), si = ld4(sin_t + at);
-        rotate_pair(a.x, c.x, co.x, si.x);
-        rotate_pair(a.y, c.y, co.y, si.y);
-        rotate_pair(a.z, c.z, co.z, si.z);
-        rotate_pair(a.w, c.w, co.w, si.w);
+    float x[VEC] = {}, y[VEC] = {};
+    if (in) {
+        load_floats<VEC>(x, row);
+        load_floats<VEC>(y, row + half);
+    }
+    if (in && r < n_heads + n_kv) {
+        float co[VEC], si[VEC];
+        load_floats<VEC>(co, cos_t + turn * half + VEC * l);
+        load_floats<VEC>(si, sin_t + turn * half + VEC * l);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) rotate_pair(x[j], y[j], co[j], si[j]);
     }
     float top = 1e-8f;
-    top = absmax_step(absmax_step(absmax_step(absmax_step(top, a.x), a.y), a.z), a.w);
-    top = absmax_step(absmax_step(absmax_step(absmax_step(top, c.x), c.y), c.z), c.w);
+#pragma unroll
+    for (int j = 0; j < VEC; ++j) top = absmax_step(absmax_step(top, x[j]), y[j]);
 #pragma unroll
     for (int o = LPR / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     if (!in) return;
     if (r < n_heads) {
-        float* o = q_out + m * q_stride + static_cast<int64_t>(r) * head_dim + 4 * l;
-        *reinterpret_cast<float4*>(o) = a;
-        *reinterpret_cast<float4*>(o + half) = c;
+        float* o = q_out + m * q_stride + static_cast<int64_t>(r) * head_dim + VEC * l;
+        store_floats<VEC>(o, x);
+        store_floats<VEC>(o + half, y);
         return;
     }
     const bool is_v = r >= n_heads + n_kv;
     const int h = r - n_heads - (is_v ? n_kv : 0);
     const int64_t at = (static_cast<int64_t>(b) * n_kv + h) * max_seq + pos;
     const float inv = __fdiv_rn(127.0f, top);
-    auto q4 = [&](const float4& v) {
-        return make_char4(quantize_code<127, -127>(v.x, inv), quantize_code<127, -127>(v.y, inv), quantize_code<127, -127>(v.z, inv),
-                          quantize_code<127, -127>(v.w, inv));
+    auto put = [&](int8_t* to, const float (&v)[VEC]) {
+        union { char4 c[VEC / 4]; uint2 w; } q;
+#pragma unroll
+        for (int j = 0; j < VEC / 4; ++j)
+            q.c[j] = make_char4(quantize_code<127, -127>(v[4 * j], inv), quantize_code<127, -127>(v[4 * j + 1], inv),
+                                quantize_code<127, -127>(v[4 * j + 2], inv), quantize_code<127, -127>(v[4 * j + 3], inv));
+        if constexpr (VEC == 8) *reinterpret_cast<uint2*>(to) = q.w;
+        else *reinterpret_cast<char4*>(to) = q.c[0];
     };
-    int8_t* codes = (is_v ? vc : kc) + at * head_dim + 4 * l;
-    *reinterpret_cast<char4*>(codes) = q4(a);
-    *reinterpret_cast<char4*>(codes + half) = q4(c);
+    int8_t* codes = (is_v ? vc : kc) + at * head_dim + VEC * l;
+    put(codes, x);
+    put(codes + half, y);
     if (l == 0) (is_v ? vs : ks)[at] = __fdiv_rn(top, 127.0f);
 }
 
 // ---- read back --------------------------------------------------------------------------------------------------------
-constexpr int kLoadThreads = 256, kLoadPerThread = 4;
+// A lane turns 8 codes of a row into 8 floats, kLoadRows times.  grid (heads * row blocks, keys | values).  WIDE: the outputs are
+// 32-byte aligned, and a lane's floats leave as one 32-byte store.
+constexpr int kLoadThreads = 256, kLoadRows = 2;
+template <bool WIDE>
 __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t* __restrict__ kc, const float* __restrict__ ks,
                                                                     const int8_t* __restrict__ vc, const float* __restrict__ vs, int64_t max_seq,
-                                                                    int head_dim, int64_t vecs, int64_t chunks, int64_t src_heads,
+                                                                    int head_dim, int rows, int chunks, int step, int64_t src_heads,
                                                                     float* __restrict__ k_out, float* __restrict__ v_out, int64_t out_max_seq,
                                                                     int64_t out_row0) {
     pdl_launch_dependents();
     pdl_wait();
-    const int64_t bh = blockIdx.x / chunks, chunk = blockIdx.x - bh * chunks;
+    const int per_row = head_dim >> 3;
+    const int64_t bh = blockIdx.x / static_cast<unsigned>(chunks);
+    const int chunk = static_cast<int>(blockIdx.x - bh * chunks);
+    const int row = threadIdx.x / per_row, col = (threadIdx.x - row * per_row) * 8;
+    if (row >= step) return;                                      // step: rows that the block's threads cover at once
     const int64_t src = (bh % src_heads) * max_seq;               // src_heads: heads of all source sequences, or of the one shared
     const bool is_v = blockIdx.y != 0;
-    const int8_t* codes = (is_v ? vc : kc) + src * head_dim;
+    const int8_t* codes = (is_v ? vc : kc) + src * head_dim + col;
     const float* scales = (is_v ? vs : ks) + src;
-    float* out = (is_v ? v_out : k_out) + (bh * out_max_seq + out_row0) * head_dim;
-    const uint32_t per_row = static_cast<uint32_t>(head_dim) / 4;
-    char4 c[kLoadPerThread];
-    float s[kLoadPerThread];
+    float* out = (is_v ? v_out : k_out) + (bh * out_max_seq + out_row0) * head_dim + col;
+    const int64_t first = static_cast<int64_t>(chunk) * (kLoadRows * step) + row;
+    uint2 c[kLoadRows];
+    float s[kLoadRows];
 #pragma unroll
-    for (int u = 0; u < kLoadPerThread; ++u) {
-        const int64_t v = (chunk * kLoadPerThread + u) * kLoadThreads + threadIdx.x;
-        if (v < vecs) {
-            c[u] = *reinterpret_cast<const char4*>(codes + 4 * v);
-            s[u] = scales[v / per_row];
+    for (int u = 0; u < kLoadRows; ++u) {
+        const int64_t r = first + u * step;
+        if (r < rows) {
+            c[u] = *reinterpret_cast<const uint2*>(codes + r * head_dim);
+            s[u] = scales[r];
         }
     }
 #pragma unroll
-    for (int u = 0; u < kLoadPerThread; ++u) {
-        const int64_t v = (chunk * kLoadPerThread + u) * kLoadThreads + threadIdx.x;
-        if (v < vecs) *reinterpret_cast<float4*>(out + 4 * v) = make_float4(c[u].x * s[u], c[u].y * s[u], c[u].z * s[u], c[u].w * s[u]);
+    for (int u = 0; u < kLoadRows; ++u) {
+        const int64_t r = first + u * step;
+        if (r >= rows) break;
+        const char4 a = *reinterpret_cast<const char4*>(&c[u].x), d = *reinterpret_cast<const char4*>(&c[u].y);
+        const float lo[4] = {a.x * s[u], a.y * s[u], a.z * s[u], a.w * s[u]}, hi[4] = {d.x * s[u], d.y * s[u], d.z * s[u], d.w * s[u]};
+        float* o = out + r * head_dim;
+        if constexpr (WIDE) {
+            store_floats<8>(o, {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]});
+        } else {
+            store_floats<4>(o, lo);
+            store_floats<4>(o + 4, hi);
+        }
     }
 }
 
@@ -959,7 +1002,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
-    static constexpr int ST = HD == 128 ? 2 : 4;
+    static constexpr int ST = (QW == 4 ? 2 : 1) * (128 / HD);
     static constexpr int kGroup = ST * Half<HD>::kBytes, kRing = KW * kGroups * kGroup;
     static constexpr int kOuts = kWarps * NQ * HD * 4;
     static constexpr int kQ = kRing > kOuts ? kRing : kOuts;
@@ -1094,7 +1137,7 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t prefix_max) {
     PrefixPlan p = {};
     const int64_t R = batch * (n_heads / n_kv);
-    p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : 0);
+    p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : (R <= 32 ? 4 : 0));
     const int64_t per_block = p.qw ? 8 * p.qw : kPrefixTcRows;
     p.blocks = static_cast<int>(ceil_div(R, per_block));
     const int64_t most = ceil_div(prefix_max, p.qw ? kTile * (kWarps / p.qw) : kPrefixTcTile);        // a tile for every group of warps
@@ -1118,6 +1161,7 @@ int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
 template <int HD>
 int launch_prefix(const DecodeArgs& a, const PrefixPlan& plan, cudaStream_t s) {
     if (plan.qw == 0) return launch_prefix_tc(a, HD, plan.splits, plan.blocks, s);
+    if (plan.qw == 4) return launch_prefix<HD, 4>(a, plan, s);
     return plan.qw == 1 ? launch_prefix<HD, 1>(a, plan, s) : launch_prefix<HD, 2>(a, plan, s);
 }
 
@@ -1301,16 +1345,28 @@ int sgqd_rope_kv_store_int8(const float* qkv, int64_t qkv_stride, int64_t t_new,
     if ((rc = check_device()) != SGQ_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t rows = n_heads + 2 * kv;
-#define SGQ_STORE(LPR)                                                                                                                    \
-    SGQ_CUDA_TRY(launch_kernel(rope_kv_store_int8_kernel<LPR>,                                                                            \
-                               dim3(static_cast<unsigned>(cache->batch * t_new), static_cast<unsigned>(ceil_div(rows, kStoreThreads / LPR))), \
-                               dim3(kStoreThreads), 0, s, true, qkv, qkv_stride, static_cast<int>(t_new), static_cast<int>(n_heads),       \
-                               static_cast<int>(kv), static_cast<int>(hd), cos_table, sin_table, table_rows, pos, pos_stride, n_new, rope_offset,       \
-                               q_out, q_stride, cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, cache->max_seq))
-    if (hd <= 32) SGQ_STORE(4);
-    else if (hd <= 64) SGQ_STORE(8);
-    else if (hd <= 128) SGQ_STORE(16);
-    else SGQ_STORE(32);
+#define SGQ_STORE(LPR, VEC)                                                                                                                \
+    do {                                                                                                                                   \
+        const int64_t blocks = ceil_div(rows * LPR, kStoreThreads), threads = ceil_div(ceil_div(rows * LPR, blocks), 32) * 32;             \
+        SGQ_CUDA_TRY(launch_kernel(rope_kv_store_int8_kernel<LPR, VEC>, dim3(static_cast<unsigned>(cache->batch * t_new),                  \
+                                   static_cast<unsigned>(ceil_div(rows * LPR, threads))), dim3(static_cast<unsigned>(threads)), 0, s,      \
+                                   true, qkv, qkv_stride, static_cast<int>(t_new), static_cast<int>(n_heads), static_cast<int>(kv),        \
+                                   static_cast<int>(hd), cos_table, sin_table, table_rows, pos, pos_stride, n_new, rope_offset, q_out,     \
+                                   q_stride, cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales, cache->max_seq));           \
+    } while (0)
+    const bool wide = hd % 16 == 0 && aligned(qkv, 32) && qkv_stride % 8 == 0 && aligned(q_out, 32) && q_stride % 8 == 0 &&
+                      aligned(cos_table, 32) && aligned(sin_table, 32);
+    if (wide) {
+        if (hd <= 32) SGQ_STORE(2, 8);
+        else if (hd <= 64) SGQ_STORE(4, 8);
+        else if (hd <= 128) SGQ_STORE(8, 8);
+        else SGQ_STORE(16, 8);
+    } else {
+        if (hd <= 32) SGQ_STORE(4, 4);
+        else if (hd <= 64) SGQ_STORE(8, 4);
+        else if (hd <= 128) SGQ_STORE(16, 4);
+        else SGQ_STORE(32, 4);
+    }
 #undef SGQ_STORE
     return SGQ_OK;
 }
@@ -1327,13 +1383,15 @@ int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_t batch,
     if (!k_out || !v_out) return bad(SGQ_ERR_NULL_POINTER, "an output is NULL");
     if ((rc = check_cache_pointers(cache)) != SGQ_OK) return rc;
     if (!aligned(k_out, 16) || !aligned(v_out, 16)) return bad(SGQ_ERR_ALIGNMENT, "outputs must be 16-byte aligned");
-    const int64_t vecs = rows * cache->head_dim / 4, chunks = ceil_div(vecs, kLoadThreads * kLoadPerThread);
+    const int64_t step = kLoadThreads / (cache->head_dim / 8), chunks = ceil_div(rows, step * kLoadRows);
     const int64_t heads = batch * cache->n_kv_heads;
     if (heads > 0x7fffffff / chunks) return bad(SGQ_ERR_BAD_SHAPE, "too many rows for one call");
     if ((rc = check_device()) != SGQ_OK) return rc;
-    SGQ_CUDA_TRY(launch_kernel(kv_load_int8_kernel, dim3(static_cast<unsigned>(heads * chunks), 2), dim3(kLoadThreads), 0,
+    const bool wide = aligned(k_out, 32) && aligned(v_out, 32);
+    SGQ_CUDA_TRY(launch_kernel(wide ? kv_load_int8_kernel<true> : kv_load_int8_kernel<false>, dim3(static_cast<unsigned>(heads * chunks), 2), dim3(kLoadThreads), 0,
                                static_cast<cudaStream_t>(stream), true, cache->k_codes, cache->k_scales, cache->v_codes, cache->v_scales,
-                               cache->max_seq, static_cast<int>(cache->head_dim), vecs, chunks, cache->batch * cache->n_kv_heads, k_out, v_out,
+                               cache->max_seq, static_cast<int>(cache->head_dim), static_cast<int>(rows), static_cast<int>(chunks),
+                               static_cast<int>(step), cache->batch * cache->n_kv_heads, k_out, v_out,
                                out_max_seq, out_row0));
     return SGQ_OK;
 }

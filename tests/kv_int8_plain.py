@@ -42,9 +42,10 @@ def decode(qkv, cache, cos, sin, pos, heads, prefix=None, prefix_len=0):
     The bound: the query's rotation rounds three times and its fixed point by half of 1 / 8355000 of its largest value, that
     is 4 * 2^-24 of that value together, and the score is rounded when it is scaled (twice), when the maximum is
     subtracted (once) and by the key's scale (once): a score is off by at most e = 8 * 2^-24 * max |q| sum |k| / sqrt(dim).
-    Weights are off by 2 e (their sum as well, hence the 2) and by the exponential (2 ulp) and their own fixed point (half an
-    ulp).  Sums over n positions round once per 32-position tile of a warp, with one rescaling each, and when warps, CTAs and
-    prefix parts are joined (at most 40 times): (3 n / 256 + 40) * 2^-24 of the largest value."""
+    Weights are off by 2 e (their sum as well, hence the 2), by the exponential (2 ulp: 4 * 2^-24) and by their own fixed point
+    (half of 1 / 4194000 of the largest: 2 * 2^-24), 6 * 2^-24 together.  Sums over n positions round once per 32-position tile of
+    a warp, with one rescaling each, and when warps, CTAs and prefix parts are joined (at most 39 times):
+    (3 n / 256 + 39) * 2^-24 of the largest value."""
     cache = {k: v.copy() for k, v in cache.items()}
     B, kv, S, dim = cache["k_codes"].shape
     G = heads // kv
@@ -72,5 +73,5 @@ def decode(qkv, cache, cos, sin, pos, heads, prefix=None, prefix_len=0):
             out[b, at] = attend(qh, *read).reshape(-1)
             e = 8 * 2.0 ** -24 * np.abs(qh).max(-1) * np.abs(read[0]).sum(-1).max() / np.sqrt(dim)            # [G]
             n = read[0].shape[0]
-            tol[b, at] = np.repeat(np.abs(read[1]).max() * (2 * e + (3 * n / 256 + 40 + 5) * 2.0 ** -24), dim)
+            tol[b, at] = np.repeat(np.abs(read[1]).max() * (2 * e + (3 * n / 256 + 39 + 6) * 2.0 ** -24), dim)
     return out, cache, tol

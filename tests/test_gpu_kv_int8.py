@@ -143,6 +143,29 @@ def test_store_reads_rows_that_are_slices_of_wider_ones(sgq):
         same_bits(other, results[0])
 
 
+@pytest.mark.parametrize("dim", [16, 32, 64, 128, 208, 256])
+def test_store_and_load_off_the_32_byte_grid(sgq, dim):
+    """Rows, tables and outputs that start 16 bytes behind a multiple of 32: the bits of the aligned ones."""
+    r = np.random.default_rng(dim)
+    B, T, heads, kv, S = 2, 9, 3, 3, 12
+    x = dev(r.standard_normal((B, T, (heads + 2 * kv) * dim)).astype(np.float32))
+    cos, sin = (dev(t) for t in plain.tables(S, dim))
+
+    def off(t):
+        o = torch.empty(t.numel() + 8, device="cuda")
+        return o[4 if o.data_ptr() % 32 == 0 else 8:][:t.numel()].view(t.shape).copy_(t)
+
+    results = []
+    for f in (lambda t: t, off):
+        cache, q = sgq.KVCacheInt8.empty(B, kv, S, dim, "cuda"), f(torch.zeros(B, T, heads * dim, device="cuda"))
+        sgq.rope_kv_store_int8(f(x), cache, f(cos), f(sin), ints(0, 3), heads, q_out=q)
+        k, v = (f(torch.zeros(B, kv, S, dim, device="cuda")) for _ in range(2))
+        assert (k.data_ptr() % 32 == 0) == (f is not off)
+        sgq.kv_load_int8(cache, S, k_out=k, v_out=v)
+        results.append({**to_host(cache), "q": q.cpu().numpy(), "k": k.cpu().numpy(), "v": v.cpu().numpy()})
+    same_bits(results[1], results[0])
+
+
 # ---- read back ------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("B,batch,kv,dim,S,rows,row0,out_rows", [
     (1, 1, 1, 128, 1, 1, 0, 1), (2, 2, 3, 64, 37, 33, 0, 33), (1, 5, 2, 128, 70, 65, 0, 65), (3, 3, 2, 8, 300, 299, 7, 310),
@@ -202,13 +225,13 @@ DECODE = [
     (1, 1, 1, 128, 1, [0]), (1, 1, 1, 64, 8, [7]), (2, 2, 2, 128, 64, [6, 0]), (1, 8, 1, 128, 70, [32]), (8, 16, 16, 128, 640, [129]),
     (3, 5, 5, 64, 333, [332, 0, 31]), (2, 12, 3, 64, 100, [63, 64]), (2, 10, 2, 128, 257, [255, 256]), (1, 14, 2, 64, 1000, [999]),
     (2, 32, 4, 128, 300, [299, 150]), (1, 16, 1, 128, 90, [33]), (1, 34, 2, 64, 50, [40]), (40, 32, 32, 64, 128, [100]),
-    (5, 4, 1, 128, 2051, [2050, -1, 17, 2051, 1024]), (1, 4, 2, 128, 9001, [9000]), (3, 24, 8, 128, 31, [-5, 30, 1]), (37, 8, 8, 64, 512, [500]), (33, 16, 16, 128, 300, [255]),
+    (5, 4, 1, 128, 2051, [2050, -1, 17, 2051, 1024]), (1, 4, 2, 128, 9001, [9000]), (3, 20, 4, 128, 31, [-5, 30, 1]), (37, 8, 8, 64, 512, [500]), (33, 16, 16, 128, 300, [255]),
     (16, 8, 4, 128, 1500, [1499 - 99 * i for i in range(16)]), (9, 40, 8, 64, 700, [699, 64, 63, 128, 127, 0, 1, -1, 300])]
 
 
 # caches that may grow long (dealt out to all warps of the device): few and many positions in them, idle slots at every place
 LONG = [
-    (1, 4, 2, 128, 80000, [70001]), (1, 16, 16, 128, 9600, [0]), (3, 8, 8, 128, 7000, [6999, 63, 64]), (2, 32, 4, 64, 20000, [127, 19999]),
+    (1, 4, 2, 128, 80000, [70001]), (1, 16, 16, 128, 9600, [0]), (3, 6, 6, 128, 7000, [6999, 63, 64]), (2, 32, 4, 64, 20000, [127, 19999]),
     (5, 8, 8, 64, 2000, [-1, 1999, -1, 128, -1]), (2, 48, 4, 128, 19000, [300, 5000]), (37, 2, 1, 64, 5000, [500]), (2, 40, 2, 128, 16000, [15999, 0]),
     (40, 4, 1, 128, 2000, [(51 * i) % 2003 - 2 for i in range(40)]), (4, 10, 2, 128, 20000, [-1, -1, -1, -1]), (33, 1, 1, 128, 3000, [255])]
 
@@ -238,7 +261,12 @@ def test_decode_with_vanishing_and_steep_scores(sgq, scale):
 PREFIX = [
     (1, 1, 1, 128, 4, [0], 1, 1), (2, 2, 2, 64, 16, [3, 15], 33, 40), (8, 16, 16, 128, 32, [9], 200, 256), (3, 12, 4, 64, 20, [0, 19, -1], 65, 65),
     (5, 8, 1, 128, 40, [39, 1, 2, 3, 40], 513, 600), (9, 14, 2, 128, 12, [4], 31, 64), (33, 4, 4, 64, 5, [2], 130, 130), (2, 16, 1, 64, 8, [7, 0], 3001, 3001),
-    (2, 4, 2, 128, 50, [49, 12], 0, 8), (2, 4, 2, 128, 50, [49, 12], -3, 8), (2, 4, 2, 128, 50, [49, 12], 99, 8), (3, 8, 8, 128, 7000, [6999, -1, 3], 700, 720), (70, 8, 2, 128, 6, [5], 90, 90)]
+    (2, 4, 2, 128, 50, [49, 12], 0, 8), (2, 4, 2, 128, 50, [49, 12], -3, 8), (2, 4, 2, 128, 50, [49, 12], 99, 8), (3, 6, 6, 128, 7000, [6999, -1, 3], 700, 720), (70, 8, 2, 128, 6, [5], 90, 90)]
+# one to 130 query rows per kv head, prefixes that end inside, at and behind a tile of 32 and of 128 positions
+PREFIX += [(2, 16, 2, 128, 40, [33, 2], n, 400) for n in (31, 32, 33, 127, 128, 129, 256, 257, 400)]
+PREFIX += [(B, 10, 10, dim, 40, [33], 300, 384) for B in (7, 8, 9, 16, 17, 24, 32, 33, 127, 128, 129) for dim in (64, 128)]
+PREFIX += [(35, 4, 2, dim, 40, [33], n, 1000) for dim in (64, 128) for n in (1, 31, 127, 128, 129, 255, 256, 1000)]
+PREFIX += [(34, 1, 1, 128, 8, [2], 20011, 20480), (130, 2, 1, 64, 8, [2], 5000, 5000), (1, 7, 1, 128, 8, [2], 20011, 20480)]
 
 
 @pytest.mark.parametrize("B,heads,kv,dim,S,pos,prefix_len,prefix_max", PREFIX)
@@ -271,6 +299,39 @@ def test_values_that_are_not_finite_reach_their_own_head_only(sgq):
             else:
                 at = slice(h * dim, (h + 1) * dim)
                 assert (np.abs(out[b, h] - clean[0][b, at]) <= clean[2][b, at]).all(), (b, h)
+
+
+@pytest.mark.parametrize("B", [2, 12, 40])              # 8 (mma.sync, one warp of rows), 48 and 160 query rows per kv head
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_that_are_not_finite_behind_a_prefix(sgq, B, dim):
+    heads, kv, S, p, P = 8, 2, 40, 30, 300
+    r = np.random.default_rng(21)
+    host, first = random_cache(r, B, kv, S, dim), random_cache(r, 1, kv, P + 20, dim, junk_from=[P])
+    qkv = r.standard_normal((B, heads + 2 * kv, dim)).astype(np.float32)
+    cos, sin = plain.tables(S + P + 20, dim)
+    clean = plain.decode(qkv.reshape(B, -1), host, cos, sin, [p], heads, first, P)
+
+    def run():
+        out = sgq.attn_decode_prefix_int8(dev(qkv.reshape(B, -1)), to_gpu(sgq, host), to_gpu(sgq, first), ints(P), dev(cos), dev(sin), ints(p), heads)
+        return out.cpu().numpy().reshape(B, heads, dim)
+
+    def check(out, bad):
+        for b in range(B):
+            for h in range(heads):
+                if bad(b, h):
+                    assert np.isnan(out[b, h]).all(), (b, h)
+                else:
+                    at = slice(h * dim, (h + 1) * dim)
+                    assert (np.abs(out[b, h] - clean[0][b, at]) <= clean[2][b, at]).all(), (b, h)
+
+    qkv[0, 1, 5], qkv[B - 1, 6, 0] = np.nan, np.inf
+    rows = {(0, 1), (B - 1, 6)}
+    check(run(), lambda b, h: (b, h) in rows)
+    for name, value, at in (("k_scales", np.inf, 7), ("k_scales", np.nan, 290), ("v_scales", np.inf, 150), ("v_scales", np.nan, 0)):
+        kept = first[name].copy()
+        first[name][0, 1, at] = value                # heads 4 to 7 of every sequence
+        check(run(), lambda b, h: h >= 4 or (b, h) in rows)
+        first[name][:] = kept
 
 
 def test_decode_and_store_hold_the_same_row(sgq):
@@ -377,7 +438,7 @@ def test_decode_steps_in_a_graph_on_a_side_stream(sgq):
 
 
 def test_two_calls_at_once_on_two_streams(sgq):
-    B, heads, kv, dim, S, P = 4, 16, 4, 128, 900, 2000
+    B, heads, kv, dim, S, P = 4, 20, 4, 128, 900, 2000
     r = np.random.default_rng(16)
     first = to_gpu(sgq, random_cache(r, 1, kv, P, dim))
     cos, sin = (dev(t) for t in plain.tables(S + P, dim))
