@@ -822,8 +822,8 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
     constexpr int ST = Shape::ST, VEC = HD / 32, STEP = Shape::kStep;
     using Attn = WarpAttention<HD, NQ, ST>;
     extern __shared__ __align__(128) uint8_t sm[];
-    pdl_launch_dependents();
     if (!PREFIX) pdl_wait();                                          // else at the end: see attn_decode_int8_kernel
+    pdl_launch_dependents();                                          // behind the wait: the joining kernel reads `pos` at once
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.n_heads / a.n_kv, units_per_seq = a.n_kv * blocks;
     const int gw = blockIdx.x * kFlatWarpsPerSm + warp;
     uint8_t* ring = sm + warp * kGroups * Shape::kGroup;

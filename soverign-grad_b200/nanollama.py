@@ -15,6 +15,10 @@ the prompt's causal attention, the embedding lookup and the greedy argmax are th
 include/sgq_decoder.h; torch supplies device memory only.  A decode step touches no host state — the
 cache position lives in device memory — so one step is recorded into a CUDA graph and replayed.
 
+Key/value cache: fp32, or with kv_cache="int8" codes of one byte with a scale per row of head_dim (KVCacheInt8): a quarter of
+the memory, and of the bytes that a decode step reads behind long contexts.  With max_prefix > 0 a prefix that all sequences
+share (set_prefix) is computed and held once, in front of every sequence's own cache.
+
 Sharding (world > 1): heads, SwiGLU columns, output features of wo / w_down and the vocabulary are
 split by column over the ranks; each split output is all-gathered over NCCL and re-interleaved
 (`sharding.ShardedLinear` has the single-layer version of the same scheme).
@@ -29,8 +33,9 @@ import torch
 import contextlib
 import ctypes as C
 
-from . import (LAYOUT_NK, PATH_AUTO, PATH_GEMV, PATH_TC_BF16, QuantizedTensor, Workspace, _ptr, _stream, check, interleave_slices, lib,
-               linear_int4_prepared, prepared_x_bytes, quantize_int4, quantized_matmul, set_stream_overlap)
+from . import (LAYOUT_NK, PATH_AUTO, PATH_GEMV, PATH_TC_BF16, KVCacheInt8, QuantizedTensor, Workspace, _ptr, _stream, attn_decode_int8,
+               attn_decode_prefix_int8, check, interleave_slices, kv_load_int8, lib, linear_int4_prepared, prepared_x_bytes, quantize_int4,
+               quantized_matmul, rope_kv_store_int8, set_stream_overlap)
 
 
 @dataclass
@@ -78,12 +83,12 @@ def default_init(cfg: NanoLlamaConfig, device, seed: int) -> Callable[[str, int]
     return make
 
 
-def rope_tables(cfg: NanoLlamaConfig, device):
-    """nn::RotaryEmbedding (nn.hpp:583-607): float32 inv_freq and theta, tables [max_seq, head_dim/2]."""
+def rope_tables(cfg: NanoLlamaConfig, device, rows: Optional[int] = None):
+    """nn::RotaryEmbedding (nn.hpp:583-607): float32 inv_freq and theta, tables [rows (max_seq), head_dim/2]."""
     half = cfg.head_dim // 2
     i = torch.arange(half, dtype=torch.float32)
     inv_freq = 1.0 / torch.pow(torch.tensor(cfg.rope_base, dtype=torch.float32), (2.0 * i) / float(cfg.head_dim))
-    theta = torch.arange(cfg.max_seq, dtype=torch.float32)[:, None] * inv_freq[None, :]
+    theta = torch.arange(cfg.max_seq if rows is None else rows, dtype=torch.float32)[:, None] * inv_freq[None, :]
     return torch.cos(theta.double()).float().to(device).contiguous(), torch.sin(theta.double()).float().to(device).contiguous()
 
 
@@ -146,7 +151,15 @@ class NanoLlamaInt4:
     def __init__(self, cfg: NanoLlamaConfig, device, batch: int, *, seed: int = 0,
                  init: Optional[Callable[[str, int], torch.Tensor]] = None, rank: int = 0, world: int = 1, group=None,
                  decode_path: int = PATH_AUTO, prefill_path: int = PATH_AUTO, overlap: int = 1,
-                 exchange: str = "peer"):
+                 exchange: str = "peer", kv_cache: str = "fp32", max_prefix: int = 0):
+        """kv_cache: "fp32" or "int8" (one GPU, heads of 64 or 128).  max_prefix: the longest shared prefix (set_prefix) that an
+        "int8" cache has room for; a sequence's own tokens have max_seq positions behind it."""
+        if kv_cache not in ("fp32", "int8"):
+            raise ValueError('kv_cache must be "fp32" or "int8"')
+        if kv_cache == "int8" and (world > 1 or cfg.head_dim not in (64, 128)):
+            raise ValueError("the int8 cache serves one GPU and heads of 64 or 128")
+        if max_prefix < 0 or (max_prefix > 0 and kv_cache != "int8"):
+            raise ValueError("a shared prefix (max_prefix > 0) needs the int8 cache")
         if cfg.n_heads % world or cfg.hidden % (32 * world) or cfg.dim % (32 * world) or cfg.vocab % (32 * world):
             raise ValueError("heads, hidden, dim and vocab must split into equal 32-row slices per rank")
         self.cfg, self.device, self.batch = cfg, torch.device(device), batch
@@ -187,11 +200,23 @@ class NanoLlamaInt4:
         self.final_norm = torch.ones(cfg.dim, device=dev)
         self.lm_head = _Linear(_rows(init("lm_head", -1).to(dev).float(), v0, v1), cfg.group, self.ws)
 
-        self.cos, self.sin = rope_tables(cfg, dev)
-        shape = (cfg.n_layers, batch, self.h_local, cfg.max_seq, hd)
-        self.k_cache = torch.zeros(shape, device=dev)
-        self.v_cache = torch.zeros(shape, device=dev)
+        self.cos, self.sin = rope_tables(cfg, dev, cfg.max_seq + max_prefix)
+        self.kv_cache, self.max_prefix = kv_cache, max_prefix
+        self.prefix_rows = 0                             # tokens of the shared prefix; prefix_len is the device's copy
+        if kv_cache == "int8":
+            caches = lambda b, rows: [KVCacheInt8.empty(b, self.h_local, rows, hd, dev) for _ in range(cfg.n_layers)]  # noqa: E731
+            self.kv, self.prefix_kv = caches(batch, cfg.max_seq), caches(1, max_prefix) if max_prefix else None
+            self.prefix_len = torch.zeros(1, dtype=torch.int32, device=dev)
+            # the attention's scratch is its own: its size never changes, so recorded steps stay valid
+            self.attn_ws = Workspace(dev)
+            flat = int(lib.sgqd_attn_decode_int8_workspace_bytes(batch, self.h_local, self.h_local, hd, cfg.max_seq))
+            self._attn_launches = (2 if flat else 1) + (1 if max_prefix else 0)
+        else:
+            shape = (cfg.n_layers, batch, self.h_local, cfg.max_seq, hd)
+            self.k_cache = torch.zeros(shape, device=dev)
+            self.v_cache = torch.zeros(shape, device=dev)
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
+        self._zero = torch.zeros(1, dtype=torch.int32, device=dev)
         self._bufs = {}
         self._graph = None
         self.tok = torch.zeros(batch, dtype=torch.int64, device=dev)
@@ -293,9 +318,10 @@ class NanoLlamaInt4:
         self._count(2 if (M > 16 or M * (K // 8) > 1024) else 1)
 
     # ---- one pass over t_new new tokens per sequence ---------------------------------------
-    def _forward(self, tokens: torch.Tensor, t_new: int, path: int) -> torch.Tensor:
-        """tokens [batch * t_new] (sequence-major).  Returns the final-normed hidden state [M, dim]."""
-        c, B = self.cfg, self.batch
+    def _forward(self, tokens: torch.Tensor, t_new: int, path: int, fill_prefix: bool = False) -> Optional[torch.Tensor]:
+        """tokens [batch * t_new] (sequence-major).  Returns the final-normed hidden state [M, dim].  fill_prefix: tokens are one
+        sequence, whose keys and values become the shared prefix's; nothing is returned."""
+        c, B = self.cfg, 1 if fill_prefix else self.batch
         M = B * t_new
         b = self._buffers(M)
         h, n = b["h"], b["n"]
@@ -309,11 +335,19 @@ class NanoLlamaInt4:
         for li, L in enumerate(self.layers):
             self._add_rmsnorm(h, delta, L["attn_norm"], n, p_dim)
             self._linear(L["qkv"], n, b["qkv"], path, p_dim)
-            kc, vc = self.k_cache[li], self.v_cache[li]
+            kc, vc = (None, None) if self.kv_cache == "int8" else (self.k_cache[li], self.v_cache[li])
             p_attn = None
             sites = self._peer(M) if self.world > 1 else None
             attn = None
-            if t_new == 1 and sites is not None:
+            if self.kv_cache == "int8":
+                if t_new == 1 and not fill_prefix:
+                    p_attn = p_dim
+                    self._decode_attention_int8(li, b["qkv"], b["attn"], p_attn)
+                else:
+                    bf16 = path in (PATH_AUTO, PATH_TC_BF16) and M >= 64
+                    if not self._prompt_attention_int8(li, b["qkv"], B, t_new, b["attn"], bf16, fill_prefix):
+                        return None
+            elif t_new == 1 and sites is not None:
                 # sharded: the kernel stores this rank's heads into every rank's full-width buffer itself
                 check(lib.sgqd_attn_decode_allgather(_ptr(b["qkv"]), 3 * self.dim_local, B, self.h_local, c.head_dim, _ptr(self.cos),
                                                      _ptr(self.sin), _ptr(kc), _ptr(vc), c.max_seq, _ptr(self.pos),
@@ -365,12 +399,42 @@ class NanoLlamaInt4:
         self._final_planes = p_dim
         return n
 
-    def _prefill_attention(self, qkv, kc, vc, T: int, out, bf16: bool = False):
-        """Causal attention of the prompt: q from the rotated qkv rows, k and v from the cache rows just written.
+    def _decode_attention_int8(self, li: int, qkv, out, planes):
+        """Rotary embedding, append to the int8 cache and attention of one new token per sequence, behind the shared prefix
+        where the model has room for one (also while it is empty: recorded steps then hold for any prefix)."""
+        kw = dict(out=out, prepared=planes, workspace=self.attn_ws)
+        if self.max_prefix:
+            attn_decode_prefix_int8(qkv, self.kv[li], self.prefix_kv[li], self.prefix_len, self.cos, self.sin, self.pos, self.h_local, **kw)
+        else:
+            attn_decode_int8(qkv, self.kv[li], self.cos, self.sin, self.pos, self.h_local, **kw)
+        self._count(self._attn_launches)
+
+    def _prompt_attention_int8(self, li: int, qkv, B: int, T: int, out, bf16: bool, fill_prefix: bool) -> bool:
+        """The prompt's tokens: stored in the int8 cache (or the prefix's), read back behind the shared prefix as the values
+        they are held as, and attended to, so that prompt and decode steps see the same keys and values.  False: the prefix's
+        last layer, behind whose keys and values nothing is wanted."""
+        c, P = self.cfg, 0 if fill_prefix else self.prefix_rows
+        cache = self.prefix_kv[li] if fill_prefix else self.kv[li]
+        rope_kv_store_int8(qkv.view(B, T, 3 * self.dim_local), cache, self.cos, self.sin, self._zero, self.h_local,
+                           rope_offset=self.prefix_len if P else None)
+        self._count()
+        if fill_prefix and li + 1 == c.n_layers:
+            return False
+        k, v = (torch.empty(B, self.h_local, P + T, c.head_dim, device=self.device) for _ in range(2))
+        if P:
+            kv_load_int8(self.prefix_kv[li], P, batch=B, k_out=k, v_out=v)
+        kv_load_int8(cache, T, k_out=k, v_out=v, row0=P)
+        self._count(2 if P else 1)
+        self._prefill_attention(qkv, k, v, T, out, bf16, B, P + T, self.prefix_len if P else self._zero)
+        return True
+
+    def _prefill_attention(self, qkv, kc, vc, T: int, out, bf16: bool = False, batch: Optional[int] = None, rows: Optional[int] = None, pos=None):
+        """Causal attention of the prompt: q from the rotated qkv rows, k and v from the cache rows just written (`rows` per
+        sequence, max_seq by default, the first of the T new ones at `pos`).
         bf16: the pass runs its linears on the bf16 tensor cores (2e-2 contract), so the attention does too."""
         fn = lib.sgqd_attn_prefill_bf16 if (bf16 and self.cfg.head_dim == 128) else lib.sgqd_attn_prefill
-        check(fn(_ptr(qkv), 3 * self.dim_local, self.batch, T, self.h_local, self.cfg.head_dim, _ptr(kc), _ptr(vc),
-                 self.cfg.max_seq, _ptr(self.pos), _ptr(out), self.dim_local, _stream()), "sgqd_attn_prefill")
+        check(fn(_ptr(qkv), 3 * self.dim_local, batch or self.batch, T, self.h_local, self.cfg.head_dim, _ptr(kc), _ptr(vc),
+                 rows or self.cfg.max_seq, _ptr(self.pos if pos is None else pos), _ptr(out), self.dim_local, _stream()), "sgqd_attn_prefill")
         self._count()
 
     def _logits(self, n_rows: torch.Tensor, path: int, planes=None) -> torch.Tensor:
@@ -398,8 +462,27 @@ class NanoLlamaInt4:
     def reset(self):
         self.pos.zero_()
 
+    def set_prefix(self, tokens: Optional[torch.Tensor]):
+        """tokens [P] int64 (P <= max_prefix) that stand in front of every sequence from now on; None or an empty tensor: none.
+        Their keys and values are computed and held once.  Sequences start anew: prefill is next.  Decode steps recorded
+        before stay valid."""
+        if not self.max_prefix:
+            raise ValueError("the model was built without room for a shared prefix (max_prefix)")
+        P = 0 if tokens is None else tokens.numel()
+        if P and (tokens.dim() != 1 or P > self.max_prefix):
+            raise ValueError("a prefix is one row of at most max_prefix tokens")
+        self._launches = 0
+        self.reset()
+        self.prefix_rows = 0
+        self.prefix_len.zero_()
+        if P:
+            with self._overlapped():
+                self._forward(tokens.to(self.device, dtype=torch.int64).contiguous(), P, self.prefill_path, fill_prefix=True)
+        self.prefix_rows = P
+        self.prefix_len.fill_(P)
+
     def prefill(self, prompt: torch.Tensor) -> torch.Tensor:
-        """prompt [batch, P] int64 at positions 0..P-1.  Returns the logits of the last position [batch, vocab]."""
+        """prompt [batch, P] int64 at positions 0..P-1 (behind the shared prefix, if there is one).  Returns the logits of the last position [batch, vocab]."""
         B, P = prompt.shape
         if B != self.batch or P > self.cfg.max_seq:
             raise ValueError("prompt shape does not fit the model's batch / max_seq")

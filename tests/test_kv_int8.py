@@ -190,3 +190,13 @@ def test_optional_arguments_are_refused(sgq):
         sgq.attn_decode_prefix_int8(**given(sgq), prefix=first, prefix_len=3)
     with pytest.raises(RuntimeError):
         sgq.attn_decode_int8(**given(sgq, qkv=torch.zeros(B, 2, WIDTH)))
+
+
+@pytest.mark.parametrize("kw", [dict(kv_cache="int4"), dict(kv_cache="int8", world=2), dict(kv_cache="int8", heads=8), dict(max_prefix=4),
+                                dict(kv_cache="int8", max_prefix=-1)])
+def test_the_decoder_refuses_caches_it_cannot_serve(sgq, kw):
+    import importlib
+    nl = importlib.import_module("sgq_b200.nanollama")
+    cfg = nl.NanoLlamaConfig(dim=256, n_layers=1, n_heads=kw.pop("heads", 2), hidden=512, vocab=512, max_seq=16)
+    with pytest.raises(ValueError):
+        nl.NanoLlamaInt4(cfg, "cpu", 1, **kw)
