@@ -19,31 +19,12 @@ namespace {
 constexpr int kMaxHeadDim = 256;
 constexpr int64_t kMaxPositions = 1ll << 30;       // of the attention: positions and strides between tiles in 32 bits
 
-// N = 4 or 8 consecutive floats, aligned to their own size
-template <int N>
-__device__ __forceinline__ void load_floats(float (&v)[N], const float* p) {
-    if constexpr (N == 8)
-        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
-                     : "l"(p)
-                     : "memory");
-    else {
-        const float4 x = *reinterpret_cast<const float4*>(p);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    }
-}
-template <int N>
-__device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
-    if constexpr (N == 8)
-        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
-                     "f"(v[6]), "f"(v[7])
-                     : "memory");
-    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-}
-
 // ---- store ------------------------------------------------------------------------------------------------------------
 // One group of LPR lanes per row (a head of q, k or v of one token); a lane owns VEC values of the first half of the row and the
 // same VEC of the second half, so that a rotary pair sits in one lane and only the absmax crosses lanes.  grid (tokens, row blocks).
+// What bounds it is memory: 8 x 512 tokens of 16 + 2 x 16 heads of 128 move 154 MB in 26.7 us, 88% of the rate of a plain copy.
+// VEC 8, where rows and tables allow 32-byte accesses, against 4: 26.3 / 28.9 us.  The row is read behind the token's check, not
+// next to it: 26.9 / 26.5 us where every token exists, 5.4 / 7.3 where 3 x 777 are padded to about half.
 constexpr int kStoreThreads = 256;                   // at most; the rows of a token are dealt out evenly to its blocks
 template <int LPR, int VEC>
 __global__ void __launch_bounds__(kStoreThreads) rope_kv_store_int8_kernel(const float* qkv, int64_t qkv_stride, int t_new, int n_heads, int n_kv,
@@ -112,7 +93,8 @@ __global__ void __launch_bounds__(kStoreThreads) rope_kv_store_int8_kernel(const
 
 // ---- read back --------------------------------------------------------------------------------------------------------
 // A lane turns 8 codes of a row into 8 floats, kLoadRows times.  grid (heads * row blocks, keys | values).  WIDE: the outputs are
-// 32-byte aligned, and a lane's floats leave as one 32-byte store.
+// 32-byte aligned, and a lane's floats leave as one 32-byte store (8 x 16 x 512 rows of 128, 84 MB: 14.7 us, 88% of the rate of a
+// plain copy; four codes and a 16-byte store per lane: 19.7; 1 / 2 / 4 rows of a shared prefix per lane: 4.75 / 4.3 / 5.1).
 constexpr int kLoadThreads = 256, kLoadRows = 2;
 template <bool WIDE>
 __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t* __restrict__ kc, const float* __restrict__ ks,
@@ -1002,6 +984,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
+    // tiles per step: 4 x 8 rows behind 16384 positions 22.6 / 24.9 us with 1 / 2, 24 x 16 behind 4096 25.8 / 24.1
     static constexpr int ST = (QW == 4 ? 2 : 1) * (128 / HD);
     static constexpr int kGroup = ST * Half<HD>::kBytes, kRing = KW * kGroups * kGroup;
     static constexpr int kOuts = kWarps * NQ * HD * 4;
@@ -1137,6 +1120,9 @@ struct PrefixPlan {
 PrefixPlan prefix_plan(int64_t batch, int64_t n_heads, int64_t n_kv, int64_t head_dim, int64_t prefix_max) {
     PrefixPlan p = {};
     const int64_t R = batch * (n_heads / n_kv);
+    // Up to 32 rows the tcgen05 kernel's 128 are mostly idle.  Measured, decode included (us, warps / tcgen05): 20 rows x 16 heads, 1024
+    // positions 15.1 / 20.2; 24 x 8, 4096 18.9 / 23.3; 24 x 16 heads of 64, 8192 24.7 / 33.5; 32 x 8, 16384 35.9 / 40.6.  More
+    // rows would take the warps a second pass over the prefix (48 x 8, 4096 on tcgen05: 21.8).
     p.qw = R <= 8 ? 1 : (R <= 16 ? 2 : (R <= 32 ? 4 : 0));
     const int64_t per_block = p.qw ? 8 * p.qw : kPrefixTcRows;
     p.blocks = static_cast<int>(ceil_div(R, per_block));

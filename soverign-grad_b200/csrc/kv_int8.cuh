@@ -85,6 +85,28 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return r;
 }
 
+// N = 4 or 8 consecutive floats, aligned to their own size
+template <int N>
+__device__ __forceinline__ void load_floats(float (&v)[N], const float* p) {
+    if constexpr (N == 8)
+        asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+                     : "l"(p)
+                     : "memory");
+    else {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    }
+}
+template <int N>
+__device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
+    if constexpr (N == 8)
+        asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]),
+                     "f"(v[6]), "f"(v[7])
+                     : "memory");
+    else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
 // Joins partial results (maximum, sum, value) of one output value
 struct Joined {
     float M, L, A;
@@ -120,8 +142,24 @@ __device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos
     rotate_values<HD>(v, c, s, lane);
 }
 
-// The rotated query as digits (at(j, d): where digit j of value d goes) and its unit, which carries 1/sqrt(HD) and log2(e).  A
-// NaN or an infinity in the query makes the unit NaN and the digits zero: every score is NaN.
+// What a rotated query is multiplied with on the way to its digits, from the bits of its largest |value|, and the unit of its
+// scores, which carries 1/sqrt(HD) and log2(e).  A NaN or an infinity in the query makes the unit NaN and the digits zero: every
+// score is NaN.
+__device__ __forceinline__ bool digits_hold(uint32_t top) { return top < 0x7F800000u && __uint_as_float(top) >= 1e-30f; }
+__device__ __forceinline__ float query_scale(uint32_t top) { return digits_hold(top) ? __fdiv_rn(kDigitRange, __uint_as_float(top)) : 0.f; }
+template <int HD>
+__device__ __forceinline__ float query_unit(uint32_t top) {
+    if (top >= 0x7F800000u) return CUDART_NAN_F;
+    return digits_hold(top) ? __fmul_rn(__fdiv_rn(__uint_as_float(top), kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f;
+}
+template <int HD>
+__device__ __forceinline__ uint32_t largest_bits(const float (&v)[HD / 32]) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
+    return __reduce_max_sync(0xffffffffu, top);
+}
+// The rotated query as digits (at(j, d): where digit j of value d goes) and its unit
 template <int HD, typename At>
 __device__ __forceinline__ void query_digits(const float (&v)[HD / 32], At at, float* unit, int lane) {
     constexpr int VEC = HD / 32;
