@@ -6,17 +6,17 @@
 //   S_j = Q_j K^T      kind::i8, 128 x 128 x HD for each digit plane j, into columns 128 j of tensor memory
 //   softmax            a thread holds a quarter of a row: 32 scores; the quarters exchange their maxima through shared memory
 //   O = (P_lo + P_hi) V     kind::f16, 128 x HD x 128 twice, into columns 384 ..: codes are exact in 16-bit floats, a weight is the
-//                      sum of two (22 bits), relative to the tile's largest value scale
+//                      sum of two (22 bits), relative to the largest of the tile and row
 // and adds O into fp32 registers once per tile: 16 additions in the tensor core between two roundings that are known.  (The
 // weights as digit planes, as in kv_int8.cu, need 384 columns for O and five more instructions per weight: 52 us for 32
-// sequences x 8 kv heads x 4 queries behind 16384 positions, decode included, where this form takes 43.  Queries as 16-bit floats
+// sequences x 8 kv heads x 4 queries behind 16384 positions, decode included, where this form takes 45.  Queries as 16-bit floats
 // would save as much again, but a score then carries the rounding of the tensor core's sums, 16 of them, where an exact one
 // has one.)  Keys are copied as they are (K-major, 128-byte-swizzled rows), values are widened on the way and read MN-major, so
 // nothing is transposed.  The next tile's scores run while a tile's weights are made, its outputs while the next scores are read.
-// What bounds it: the softmax between the products, 4900 cycles a tile of which the MMAs take 1800 behind it; sixteen warps in
+// What bounds it: the softmax between the products, 5000 cycles a tile of which the MMAs take 1800 behind it; sixteen warps in
 // step, so that exponentials, conversions and shared memory (which the MMAs' operands alone hold for 1800 cycles) take turns.
 // Measured without effect: products issued by several warps or a few at a time, one more warp to issue them (96 registers are
-// too few), magic-number conversions of the digits; packed fp32 arithmetic took 44.2 us to 43.3.
+// too few), magic-number conversions of the digits; packed fp32 arithmetic took 44.2 us to 43.3, the weights' unit by row 43.3 to 45.
 #include <cuda_fp16.h>
 
 #include <type_traits>
@@ -42,14 +42,14 @@ constexpr int kThreads = 512, kRows = kPrefixTcRows, kTile = kPrefixTcTile;
 constexpr int kPlane = 128 * 128;              // an operand: 128 rows of 128 bytes
 constexpr int kTmemCols = 512;
 constexpr float kAhead = 6.0f;                 // see WarpAttention in kv_int8.cu
-constexpr float kWeightScale = 256.0f;         // of weights before they are split: at most 2^14 then, and exact down to 2^-24
+constexpr int kWeightBits = 13;                // a row's weights reach about 2^13 before they are split: below the largest 16-bit float
 
 template <int HD>
 struct Shape {
     static constexpr int kVBytes = kTile * HD * 2;                    // values in 16 bits: [half of the positions][64 values][64 positions]
     static constexpr int kPPlane = kRows * kTile * 2;                 // weights in 16 bits: [half of the positions][row][64 positions]
     static constexpr int kQ = 0, kK = kQ + 3 * kPlane, kV = kK + 2 * kPlane, kP = kV + 2 * kVBytes, kSmall = kP + 2 * kPPlane;
-    static constexpr int kFloats = 128 + 4 * kTile + 4 * kRows + 8;  // units, key and value scales (twice), the quarters' maxima, tiles' value units
+    static constexpr int kFloats = 128 + 6 * kTile + 8 * kRows + 8;  // units, scales of keys, values, log2 of these (twice), maxima, tiles' value units
     static constexpr int kBars = kSmall + kFloats * 4, kBytes = kBars + 32 + 1024;   // 1024: alignment of the base
     static_assert(kBytes <= 227 * 1024 && 2 * kPPlane >= kRows * HD * 4, "shared memory");
 };
@@ -141,8 +141,9 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     float* sm_unit = reinterpret_cast<float*>(sm + S::kSmall);
     float* sm_ks = sm_unit + 128;                                     // [2][kTile]
     float* sm_vs = sm_ks + 2 * kTile;                                 // [2][kTile], relative to the tile's largest
-    float* sm_top = sm_vs + 2 * kTile;                                // [4][128]
-    float* sm_vtop = sm_top + 4 * kRows;                              // [4]: the largest of 32 value scales
+    float* sm_lv = sm_vs + 2 * kTile;                                 // [2][kTile]: log2 of these
+    float2* sm_top = reinterpret_cast<float2*>(sm_lv + 2 * kTile);    // [4][128]: a quarter's largest score, and score + sm_lv
+    float* sm_vtop = reinterpret_cast<float*>(sm_top + 4 * kRows);    // [4]: the largest of 32 value scales
     float* sm_vunit = sm_vtop + 4;                                    // [4]: what a tile's outputs are scaled by, of tile i in i % 4
     uint64_t* bars = reinterpret_cast<uint64_t*>(sm + S::kBars);      // scores done, outputs done
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2);
@@ -239,9 +240,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             if (lane == 0) sm_vtop[i >> 5] = __uint_as_float(of_warp);
             named_barrier_sync(5, kTile);
             const float top = fmaxf(fmaxf(sm_vtop[0], sm_vtop[1]), fmaxf(sm_vtop[2], sm_vtop[3]));
-            const float per = top < 1e-30f ? 0.f : __fdiv_rn(kWeightScale, top);
-            sm_vs[slot * kTile + i] = i < left ? (finite ? scale * per : CUDART_NAN_F) : 0.f;
-            if (i == 0) sm_vunit[i_tile & 3] = top * (1.0f / kWeightScale);
+            const float per = top < 1e-30f ? 0.f : __fdiv_rn(1.0f, top);
+            const float v = i < left && finite ? scale * per : 0.f;
+            sm_vs[slot * kTile + i] = i < left && !finite ? CUDART_NAN_F : v;
+            sm_lv[slot * kTile + i] = __log2f(fabsf(v));              // -inf where nothing is added
+            if (i == 0) sm_vunit[i_tile & 3] = top;
         }
     };
     if (t0 < t1) {
@@ -304,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     const int row = (warp & 3) * 32 + lane, h = warp >> 2;            // this thread: quarter h of the row
     const uint32_t tmem_row = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16);
     const float qu = sm_unit[row];
-    float m = -CUDART_INF_F;
+    float m = -CUDART_INF_F, unit = 0.f;                              // unit: of the last tile's weights
     float2 l2 = both(0.f), o[COLS / 2];
 #pragma unroll
     for (int d = 0; d < COLS / 2; ++d) o[d] = both(0.f);
@@ -330,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     };
     auto add_outputs = [&](int i_tile) {
         tcgen05_fence_after();
-        const float vunit = sm_vunit[i_tile & 3];
+        const float vunit = sm_vunit[i_tile & 3] * unit;
 #pragma unroll
         for (int q = 0; q < COLS / 16; ++q) {
             int s0[16];
@@ -373,10 +376,16 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
                 if (KEYS * h + x + 1 >= left) c[x / 2].y = -CUDART_INF_F;
             }
         }
+        float most = -CUDART_INF_F;                                   // log2 of the row's largest weight, as top is of exp2(score)
 #pragma unroll
-        for (int x = 0; x < KEYS / 2; ++x) top = fmaxf(top, fmaxf(c[x].x, c[x].y));
+        for (int x = 0; x < KEYS / 2; x += 2) {
+            const float4 lv = *reinterpret_cast<const float4*>(sm_lv + slot * kTile + KEYS * h + 2 * x);
+            const float2 w = fma2(c[x], both(qu), make_float2(lv.x, lv.y)), z = fma2(c[x + 1], both(qu), make_float2(lv.z, lv.w));
+            top = fmaxf(top, fmaxf(fmaxf(c[x].x, c[x].y), fmaxf(c[x + 1].x, c[x + 1].y)));
+            most = fmaxf(most, fmaxf(fmaxf(w.x, w.y), fmaxf(z.x, z.y)));
+        }
         top *= qu;
-        sm_top[h * kRows + row] = top;
+        sm_top[h * kRows + row] = make_float2(top, most);
         if (!fine) *gave_up = 1;
         asm volatile("cp.async.wait_group 0;" ::: "memory");
         fence_proxy_async_smem();
@@ -394,7 +403,11 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             add_outputs(i_tile - 1);
         }
 #pragma unroll
-        for (int x = 0; x < 4; ++x) top = fmaxf(top, sm_top[x * kRows + row]);
+        for (int x = 0; x < 4; ++x) {
+            const float2 other = sm_top[x * kRows + row];
+            top = fmaxf(top, other.x);
+            most = fmaxf(most, other.y);
+        }
         if (top > m + kAhead) {
             const float mn = fmaxf(m, top), corr = exp2_approx(m - mn);
             m = mn;
@@ -402,7 +415,14 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
 #pragma unroll
             for (int d = 0; d < COLS / 2; ++d) o[d] = mul2(o[d], both(corr));
         }
+        // The weights are taken times a power of two that brings the row's largest to about 2^13.  (Relative to the tile's largest
+        // value scale alone, rows that look past this tile would keep few bits of it: beside a token that takes the weight and
+        // has small values, the outputs live on weights of 2^-17.)
         const float ref = m == -CUDART_INF_F ? 0.f : m;
+        const int up = kWeightBits - __float2int_rn(fminf(fmaxf(most - ref, -100.f), 100.f));
+        const float shifted = static_cast<float>(up) - ref;
+        unit = __int_as_float((127 - up) << 23);
+        float2 sum = both(0.f);
         auto weights = [&](auto whole) {                              // whole: the tile has all its positions
 #pragma unroll
             for (int q = 0; q < KEYS / 8; ++q) {
@@ -410,12 +430,12 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     const int x = 4 * q + y;
-                    float2 p = fma2(c[x], both(qu), both(-ref));
+                    float2 p = fma2(c[x], both(qu), both(shifted));
                     p.x = exp2_approx(p.x);
                     p.y = exp2_approx(p.y);
                     if (!whole.value && KEYS * h + 2 * x >= left) p.x = 0.f;              // whatever the unit is
                     if (!whole.value && KEYS * h + 2 * x + 1 >= left) p.y = 0.f;
-                    l2 = add2(l2, p);
+                    sum = add2(sum, p);
                     const float4 v4 = *reinterpret_cast<const float4*>(sm_vs + slot * kTile + KEYS * h + 2 * (x & ~1));
                     split_weights(mul2(p, y & 1 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y)), hi[y], lo[y]);
                 }
@@ -426,6 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
         };
         if (left >= kTile) weights(std::true_type{});
         else weights(std::false_type{});
+        l2 = fma2(sum, both(unit), l2);
         if (left > kTile) {
             store_values(i_tile + 1, left - kTile);
             if (left > 2 * kTile) load_values(t + 2 * kTile);
@@ -449,7 +470,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     const float l = l2.x + l2.y;
-    sm_top[h * kRows + row] = l;
+    float* sm_sum = reinterpret_cast<float*>(sm_top);                // [4][128]
+    sm_sum[h * kRows + row] = l;
     __syncthreads();
     if (r0 + row < R) {
         float* out = a.part_o + ((static_cast<int64_t>(hk) * R + r0 + row) * splits + split) * HD + COLS * h;
@@ -459,7 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     if (h == 0 && r0 + row < R) {
         const int64_t to = (static_cast<int64_t>(hk) * R + r0 + row) * splits + split;
         a.part_ml[2 * to] = m;
-        a.part_ml[2 * to + 1] = (l + sm_top[kRows + row]) + (sm_top[2 * kRows + row] + sm_top[3 * kRows + row]);
+        a.part_ml[2 * to + 1] = (l + sm_sum[kRows + row]) + (sm_sum[2 * kRows + row] + sm_sum[3 * kRows + row]);
     }
     tcgen05_fence_before();
     __syncthreads();

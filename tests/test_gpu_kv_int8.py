@@ -334,6 +334,54 @@ def test_values_that_are_not_finite_behind_a_prefix(sgq, B, dim):
         first[name][:] = kept
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("B,heads,kv,S,P", [(2, 4, 2, 400, 0), (2, 4, 1, 9600, 0), (2, 4, 2, 40, 700), (8, 4, 1, 40, 700), (12, 8, 2, 40, 700)])
+def test_outputs_beside_a_token_that_takes_the_weight(sgq, B, heads, kv, S, P, dim):
+    """The first token of each sequence (of the prefix, where there is one) has nearly all the weight and values of next to nothing;
+    what the others leave, e^-20 times their values each, has to keep its precision: tests/kv_int8_plain.py's bound, but relative
+    to sum w |v| / sum w in the place of max |v|.  The other tokens weigh the same, so a weight's fixed point, relative to the
+    largest around it, is relative to the weight."""
+    r = np.random.default_rng(B + S + P)
+    pos = S - 7
+    cos, sin = plain.tables(S + P, dim)
+    q = r.standard_normal(dim).astype(np.float32)
+    qkv = np.zeros((B, heads + 2 * kv, dim), np.float32)
+    qkv[:, :heads] = q
+    qkv[:, heads + kv:] = r.standard_normal((B, kv, dim))
+    turned = plain.turned(q, cos[P + pos], sin[P + pos])
+    sink = turned * np.float32(20 * np.sqrt(dim) / (turned.astype(np.float64) ** 2).sum())
+
+    def held(batch, rows, with_sink):
+        c, k = {}, np.zeros((batch, kv, rows, dim), np.float32)
+        v = r.standard_normal((batch, kv, rows, dim)).astype(np.float32)
+        if with_sink:
+            k[:, :, 0], v[:, :, 0] = sink, v[:, :, 0] * 1e-12
+        c["k_codes"], c["k_scales"] = plain.held(k)
+        c["v_codes"], c["v_scales"] = plain.held(v)
+        return c
+
+    own, first = held(B, S, P == 0), held(1, P, True) if P else None
+    want, _, tol = plain.decode(qkv.reshape(B, -1), own, cos, sin, [pos], heads, first, P)
+    size = {}
+    for name, c in (("own", own), ("first", first)):
+        size[name] = None if c is None else {**c, "v_codes": np.abs(c["v_codes"])}
+    positive = np.abs(qkv)
+    positive[:, :heads + kv] = qkv[:, :heads + kv]
+    weighed, _, _ = plain.decode(positive.reshape(B, -1), size["own"], cos, sin, [pos], heads, size["first"], P)
+    most = np.zeros_like(tol)                                         # max |v|, by which tol is made
+    for b in range(B):
+        for h in range(heads):
+            hk = h // (heads // kv)
+            v = [np.abs(c["v_codes"][i, hk, :n].astype(np.float64) * c["v_scales"][i, hk, :n, None]).max()
+                 for c, i, n in ((own, b, pos), (first, 0, P)) if c is not None and n] + [np.abs(plain.held(qkv[b, heads + kv + hk])[0] / 127.0).max() * np.abs(qkv[b, heads + kv + hk]).max()]
+            most[b, h * dim:(h + 1) * dim] = max(v)
+    args = (dev(qkv.reshape(B, -1)), to_gpu(sgq, own))
+    rest = (dev(cos), dev(sin), ints(pos), heads)
+    got = sgq.attn_decode_prefix_int8(*args, to_gpu(sgq, first), ints(P), *rest) if P else sgq.attn_decode_int8(*args, *rest)
+    off = np.abs(got.cpu().numpy() - want) / (tol / most * weighed)
+    assert (weighed < 0.02 * most).all() and off.max() <= 1, off.max()
+
+
 def test_decode_and_store_hold_the_same_row(sgq):
     """A token appended by the decode step and by the prompt's store: the same bits; and the rows read back."""
     B, heads, kv, dim, S = 4, 8, 4, 128, 33
