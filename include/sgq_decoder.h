@@ -1,7 +1,7 @@
 /*
  * sgq_decoder.h — the fp32 operators that sit between the quantized linears of a LLaMA-style
  * decoder block (RMSNorm, rotary embedding + KV-cache store, single-query attention over the
- * cache, SiLU gate), exported from the same library as sgq.h.
+ * cache, SiLU gate), and the INT8 form of that cache, exported from the same library as sgq.h.
  *
  * They exist so that a whole greedy-decode step (sixteen blocks, ~200 launches) can be recorded
  * into one CUDA graph and replayed without host work: every quantity that changes from step to
@@ -18,6 +18,10 @@
  *   sgqd_silu_mul        nn::SwiGLU gate                    include/sovereigngrad/nn.hpp:151-156
  *                        simd::vec_silu                     include/sovereigngrad/simd.hpp:103-108
  *   sgqd_embedding       sovereigngrad::embedding           src/ops.cpp:2624-2659
+ *   sgqd_rope_kv_store_int8, sgqd_kv_load_int8, sgqd_attn_decode_int8, sgqd_attn_decode_prefix_int8
+ *                        rotary_embedding and CausalSelfAttention as above over keys and values
+ *                        that are held as quantization::quantize_int8 holds a row
+ *                        (src/quantization.cpp:22-78)
  *   sgqd_argmax_rows     greedy choice in NanoLLaMA::generate  include/sovereigngrad/models.hpp:291-298
  *
  * Conventions are those of sgq.h: device pointers owned by the caller, `stream` is a cudaStream_t
@@ -157,10 +161,10 @@ SGQ_API int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_
  * k_t and v_t being the values the cache then holds, the new token's included.  qkv is read only.  A sequence whose pos lies
  * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  A NaN or an infinity in a query
  * gives NaN in its head's output, and so does a row with a scale that is not finite; rows at positions behind pos are not
- * read.  The query and the softmax weights enter exact integer products as 24-bit fixed point (the query relative to its
- * largest value, the weights relative to the largest of every 32 positions), sums are fp32: errors are those of an fp32
- * evaluation.  table_rows >= max_seq.  head_dim must be 64 or 128, max_seq at most
- * 2^30.  prepared_out: as for sgqd_attn_decode.  workspace: as many bytes as the query says (0: none is read; caches that
+ * read.  The query enters exact integer products as 24-bit fixed point relative to its largest value, the softmax weights
+ * as 23-bit fixed point relative to the largest of 32 to 128 positions (behind a prefix also as the sum of two 16-bit
+ * floats, 22 bits), sums are fp32: errors are those of an fp32 evaluation.  table_rows >= max_seq.  head_dim must be 64 or
+ * 128, max_seq at most 2^30.  out may not overlap qkv.  prepared_out: as for sgqd_attn_decode.  workspace: as many bytes as the query says (0: none is read; caches that
  * may grow long need some), 256-byte aligned; it holds nothing from one call to the next, and calls that may run at the
  * same time need one each.  The query's answer follows from the sizes alone. */
 SGQ_API size_t sgqd_attn_decode_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
