@@ -635,6 +635,9 @@ struct DecodeShape {
     static constexpr int kNew = (kSmall + (NQ + 2 * kRecv + 2 * kDecodeWarps * NQ) * 4 + 15) / 16 * 16;
     static constexpr int kBytes = kNew + NewRows<HD>::kBytes;
 };
+// What bounds it: bytes where caches are long (32 x 8 kv heads x 4 queries, up to 8192 positions, 287 MB: 54.3 us, 0.81 of the rate of
+// a plain copy; all of 4096: 49.8, 0.85), a chain of latencies where they are short: position, cosines, digits, first tile,
+// merge (1 x 16 heads, 130 positions: 5.3 us; 8 x 16, 576: 8.1).
 // PER_SM: CTAs that an SM has to hold.  With three the kernel keeps within 168 registers, where the compiler spills a few that it
 // needs at the end; with 2 it uses 175.
 template <int HD, int NQ, bool PREFIX, int PER_SM>
@@ -769,6 +772,9 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
 // each unit it touches.  How many steps a unit has follows from `pos` alone, so every warp (and the kernel that joins the
 // results) finds its place by itself: nothing is handed out at run time and the result does not depend on timing.
 // The partial result of warp w for unit u goes to slot w + u: from one part of the row to the next w or u grows.
+// What bounds it: bytes; 11 us are spent around a stream that runs at the rate of a plain copy (1 x 8 kv heads x 4 queries: 131072
+// positions 53.2 us with the joining kernel, each further 131072 another 42.2).  A warp with a ring of its own, one CTA of 8 per SM:
+// 201 KB of tiles under way, no barrier between warps.
 constexpr int kFlatWarpsPerSm = 8, kFlatWarps = kSms * kFlatWarpsPerSm;
 template <int HD, int NQ>
 struct FlatShape {
@@ -934,17 +940,18 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
     if (PREFIX) pdl_wait();
 }
 
+constexpr int kJoinWarps = 16;         // of a block (8 / 16 / 32: 1 x 8 heads, 131072 positions 54.6 / 53.2 / 53.6 us, 16384 16.6 / 15.5 / 14.9)
 // Joins the partial results of attn_flat_int8_kernel (and of a prefix).  WIDE: a block per (sequence, query head), whose warps take
 // the slots in turn; else a warp per (sequence, query head).  A lane holds HD / 32 values.  Where the slots are follows from
 // `pos`, which is older than the kernel in front: that is worked out before its results are waited for.
 template <int HD, int NQ, bool WIDE, bool PREFIX>
-__global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const DecodeArgs a, int blocks) {
-    constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, BY = WIDE ? kWarps : 1;
-    __shared__ float sm_ml[kWarps][2];
-    __shared__ __align__(16) float sm_o[kWarps][HD];
+__global__ void __launch_bounds__((WIDE ? kJoinWarps : kWarps) * 32) attn_flat_join_kernel(const DecodeArgs a, int blocks) {
+    constexpr int VEC = HD / 32, STEP = FlatShape<HD, NQ>::kStep, W = WIDE ? kJoinWarps : kWarps, BY = WIDE ? W : 1;
+    __shared__ float sm_ml[W][2];
+    __shared__ __align__(16) float sm_o[W][HD];
     pdl_launch_dependents();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, G = a.n_heads / a.n_kv, units_per_seq = a.n_kv * blocks;
-    const int64_t bh = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+    const int64_t bh = WIDE ? blockIdx.x : static_cast<int64_t>(blockIdx.x) * W + warp;
     const bool there = bh < static_cast<int64_t>(a.batch) * a.n_heads;
     const int b = there ? static_cast<int>(bh / a.n_heads) : 0, h = there ? static_cast<int>(bh - static_cast<int64_t>(b) * a.n_heads) : 0;
     const int hk = h / G, g = h - hk * G, j = hk * blocks + g / NQ;
@@ -968,7 +975,7 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
         __syncthreads();
         if (warp != 0) return;
         t = JoinedHead<HD>();
-        t.template join<4>(kWarps, [&](int u, float& m, float& l, float (&v)[VEC]) {
+        t.template join<4>(W, [&](int u, float& m, float& l, float (&v)[VEC]) {
             m = sm_ml[u][0];
             l = sm_ml[u][1];
             JoinedHead<HD>::load(&sm_o[u][lane * VEC], v);
@@ -981,6 +988,8 @@ __global__ void __launch_bounds__(kWarps * 32) attn_flat_join_kernel(const Decod
 // Partial attention of every sequence's queries to the shared prefix.  grid (kv heads, splits of the prefix, blocks of 8 QW rows),
 // the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; the QW warps of a group
 // take the same tiles, which they fetch together into the group's ring, and the KW = 8 / QW groups take alternate tiles.
+// What bounds it: the s8 products of mma.sync, 8 cycles each on an SM's quarter, from 16 rows on (32 rows x 8 heads behind 16384
+// positions: 35.4 us with the decode behind it); below, start, digits and the hand-over (8 rows x 16 heads behind 2048: 11.7).
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
@@ -1219,7 +1228,7 @@ int launch_decode(const DecodeArgs& a, const DecodePlan& plan, cudaStream_t s) {
         const int64_t heads = static_cast<int64_t>(a.batch) * a.n_heads;
         // a head has about kFlatWarps / units slots: with more than a warp asks for at once, a block takes it
         if (plan.units * 6 < kFlatWarps)
-            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, true, PREFIX>, dim3(static_cast<unsigned>(heads)), dim3(kWarps * 32), 0, s, true, a, plan.blocks));
+            SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, true, PREFIX>, dim3(static_cast<unsigned>(heads)), dim3(kJoinWarps * 32), 0, s, true, a, plan.blocks));
         else
             SGQ_CUDA_TRY(launch_kernel(attn_flat_join_kernel<HD, NQ, false, PREFIX>, dim3(static_cast<unsigned>(ceil_div(heads, kWarps))), dim3(kWarps * 32), 0, s, true,
                                        a, plan.blocks));
