@@ -178,7 +178,7 @@ SGQ_API int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t 
  * prefix->max_seq), whose rows lie once in `prefix`, a cache of one sequence with the same heads: every query attends to
  * the prefix rows and to its own rows 0 .. pos[b], which stand at positions *prefix_len + t of its sequence (the rotation of
  * the new token included; table_rows >= prefix->max_seq + max_seq).  The prefix is read once for the whole
- * batch.  workspace: as for sgqd_attn_decode_int8 (0 bytes only for sizes that are refused). */
+ * batch and shares no memory with `cache`.  workspace: as for sgqd_attn_decode_int8 (0 bytes only for sizes that are refused). */
 SGQ_API size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                                                             int64_t max_seq, int64_t prefix_max);
 SGQ_API int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,

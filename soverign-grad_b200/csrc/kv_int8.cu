@@ -1116,6 +1116,14 @@ int check_cache_pointers(const sgqd_cache_int8* c) {
         return bad(SGQ_ERR_ALIGNMENT, "codes must be 16-byte aligned");
     return SGQ_OK;
 }
+// Do `rows` rows of wx floats, sx apart, and of wy floats, sy apart, share memory?  (Columns of one wider matrix do not.)
+bool rows_overlap(const float* x, int64_t sx, int64_t wx, const float* y, int64_t sy, int64_t wy, int64_t rows) {
+    const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x) / 4), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y) / 4);
+    if (a + (rows - 1) * sx + wx <= b || b + (rows - 1) * sy + wy <= a) return false;
+    if (sx != sy || rows == 1) return true;
+    const int64_t d = ((b - a) % sx + sx) % sx;
+    return d < wx || d + wy > sx;
+}
 CacheView view(const sgqd_cache_int8* c) { return CacheView{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->max_seq}; }
 
 // Splits of a shared prefix and rows per block of its kernel: a function of the sizes alone, so that the workspace's size is one
@@ -1278,6 +1286,8 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
     if ((rc = check_cache_pointers(cache)) != SGQ_OK || (prefix && (rc = check_cache_pointers(prefix)) != SGQ_OK)) return rc;
     if (!aligned(qkv, 16) || (qkv_stride & 3) || !aligned(cos_table, 16) || !aligned(sin_table, 16))
         return bad(SGQ_ERR_ALIGNMENT, "qkv rows and tables must be 16-byte aligned");
+    if (rows_overlap(qkv, qkv_stride, (n_heads + 2 * kv) * hd, out, out_stride, n_heads * hd, batch))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "out overlaps qkv");
     PreparedLayout L = {};
     if ((rc = check_prepared(prepared_out, prepared_bytes, batch, n_heads * hd, &L)) != SGQ_OK) return rc;
     const DecodePlan plan = decode_plan(batch, n_heads, kv, hd, cache->max_seq);
@@ -1337,6 +1347,8 @@ int sgqd_rope_kv_store_int8(const float* qkv, int64_t qkv_stride, int64_t t_new,
     if ((rc = check_cache_pointers(cache)) != SGQ_OK) return rc;
     if (!aligned(qkv, 16) || (qkv_stride & 3) || !aligned(q_out, 16) || (q_stride & 3) || !aligned(cos_table, 16) || !aligned(sin_table, 16))
         return bad(SGQ_ERR_ALIGNMENT, "rows and tables must be 16-byte aligned");
+    if (q_out != qkv && rows_overlap(qkv, qkv_stride, (n_heads + 2 * kv) * hd, q_out, q_stride, n_heads * hd, cache->batch * t_new))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "q_out overlaps qkv and is not qkv itself");
     if ((rc = check_device()) != SGQ_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t rows = n_heads + 2 * kv;

@@ -11,7 +11,7 @@ def sgq():
     return load_package()
 
 
-ONE, TWO, ODD = C.c_void_p(256), C.c_void_p(512), C.c_void_p(260)      # never dereferenced: validation comes first
+ONE, TWO, ODD = C.c_void_p(256), C.c_void_p(1 << 20), C.c_void_p(260)      # never dereferenced: validation comes first
 
 
 def cache(sgq, batch=2, kv=2, max_seq=16, dim=128, k=256, ks=256, v=256, vs=256):
@@ -78,6 +78,18 @@ def test_decode_arguments(sgq, prefix):
     assert call(c=cache(sgq, vs=None)) == 1 and call(c=cache(sgq, v=264)) == 6 and call(qkv=ODD) == 6 and call(stride=1025) == 6 and call(sin=ODD) == 6
     assert call(planes=ONE, nb=16) == 5 and call(c=cache(sgq, batch=17), planes=ONE, nb=1 << 20) == 4
     assert call(c=cache(sgq, batch=0, k=None), out=None) == 0
+
+
+@pytest.mark.parametrize("at,stride,overlaps", [
+    (1020, 1600, True), (-508, 1600, True), (1600, 1600, True), (1500, 1600, True),          # the same rows' columns, the next row's, over a row's end
+    (1024, 1600, False), (1088, 1600, False), (2624, 1600, False), (-512, 1600, False),      # behind the columns, or in front
+    (1024, 1604, True), (2624, 1604, False), (-512 - 1604, 1604, False)])                    # spaced otherwise
+def test_outputs_that_overlap_the_rows_they_are_made_of(sgq, at, stride, overlaps):
+    """Two rows of 1024 floats, 1600 apart, outputs `at` floats behind.  What does not overlap comes as far as the next check."""
+    qkv, out = C.c_void_p(1 << 20), C.c_void_p((1 << 20) + 4 * at)
+    if overlaps:                       # (nothing would refuse the others, on a GPU)
+        assert store(sgq, cache(sgq), qkv=qkv, stride=1600, q=out, qs=stride) == 3
+    assert decode(sgq, cache(sgq), qkv=qkv, stride=1600, out=out, os=stride, planes=ONE, nb=16) == (3 if overlaps else 5)
 
 
 def test_prefix_arguments(sgq):
