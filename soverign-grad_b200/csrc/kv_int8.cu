@@ -497,16 +497,17 @@ struct HeldRow {
 template <int HD>
 struct NewRows {
     static constexpr int kBytes = 2 * HD + 16;                             // codes of the key and of the value, their scales
-    static __device__ __forceinline__ void make(const DecodeArgs& a, int b, int hk, const float* cos_row, const float* sin_row, uint8_t* keep, int64_t row,
-                                                bool append, int lane) {
-        constexpr int VEC = HD / 32;
+    static constexpr int VEC = HD / 32;
+    static __device__ __forceinline__ void load(const DecodeArgs& a, int b, int hk, float (&x)[VEC], float (&y)[VEC], int lane) {
         const float* from = a.qkv + b * a.qkv_stride + static_cast<int64_t>(a.n_heads + hk) * HD + lane * VEC;
-        float x[VEC], y[VEC];
 #pragma unroll
         for (int j = 0; j < VEC; ++j) {
             x[j] = from[j];
             y[j] = from[static_cast<int64_t>(a.n_kv) * HD + j];
         }
+    }
+    static __device__ __forceinline__ void make(const DecodeArgs& a, float (&x)[VEC], float (&y)[VEC], const float* cos_row, const float* sin_row,
+                                                uint8_t* keep, int64_t row, bool append, int lane) {
         rotate_row<HD>(x, cos_row, sin_row, lane);
         HeldRow<HD> k, v;
         k.make(x);
@@ -686,6 +687,8 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
     for (int i = 0; i < QPW; ++i)
 #pragma unroll
         for (int j = 0; j < VEC; ++j) qv[i][j] = warp + i * W < nq ? row[(warp + i * W) * HD + j] : 0.f;
+    float new_k[VEC], new_v[VEC];
+    if (warp == W - 1) NewRows<HD>::load(a, b, hk, new_k, new_v, lane);
     const int64_t pos = a.pos[b * a.pos_stride];
     const bool live = pos >= 0 && pos < a.own.max_seq;
     const int64_t P = PREFIX ? prefix_rows(a) : 0;
@@ -698,10 +701,12 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
         rotate_row<HD>(qv[i], cos_row, sin_row, lane);
         query_planes<HD>(qv[i], sm_q + (warp + i * W) * Attn::kQueryBytes, sm_unit + warp + i * W, lane);
     }
-    // The warp that takes the last tile stores the new token's rows (in one query block of the group).
-    const bool owner = n > 0 && (n - 1) / STEP % (S * W) == split * W + warp;
+    // The CTA whose warp takes the last tile makes the new token's rows (and stores them, in one query block of the group): its last
+    // warp, which has no query of its own where the group has fewer than four.
+    const int last_warp = n > 0 ? (n - 1) / STEP % (S * W) - split * W : -1;
+    const bool owner = last_warp == warp;
     uint8_t* fresh = sm + Shape::kNew;
-    if (owner) NewRows<HD>::make(a, b, hk, cos_row, sin_row, fresh, base + pos, blockIdx.y == 0, lane);
+    if (warp == W - 1 && last_warp >= 0 && last_warp < W) NewRows<HD>::make(a, new_k, new_v, cos_row, sin_row, fresh, base + pos, blockIdx.y == 0, lane);
     __syncthreads();
     Attn w;
     w.init(lane);
@@ -899,9 +904,12 @@ __global__ void __launch_bounds__(kFlatWarpsPerSm * 32) attn_flat_int8_kernel(co
                     rotate_row<HD>(qv[q], a.cos_t + turn, a.sin_t + turn, lane);
                     query_planes<HD>(qv[q], sm_q + q * Attn::kQueryBytes, sm_unit + q, lane);
                 }
-                if (use.s + left >= use.T)                                 // the run holds the unit's last step
-                    NewRows<HD>::make(a, use.b, hk, a.cos_t + turn, a.sin_t + turn, fresh,
+                if (use.s + left >= use.T) {                               // the run holds the unit's last step
+                    float x[VEC], y[VEC];
+                    NewRows<HD>::load(a, use.b, hk, x, y, lane);
+                    NewRows<HD>::make(a, x, y, a.cos_t + turn, a.sin_t + turn, fresh,
                                       (static_cast<int64_t>(use.b) * a.n_kv + hk) * a.own.max_seq + use.n - 1, qb == 0, lane);
+                }
                 __syncwarp();
                 w.init(lane);
                 w.use_queries(sm_q, sm_unit);
