@@ -638,7 +638,7 @@ struct DecodeShape {
 };
 // What bounds it: bytes where caches are long (32 x 8 kv heads x 4 queries, up to 8192 positions, 287 MB: 54.3 us, 0.81 of the rate of
 // a plain copy; all of 4096: 49.8, 0.85), a chain of latencies where they are short: position, cosines, digits, first tile,
-// merge (1 x 16 heads, 130 positions: 5.3 us; 8 x 16, 576: 8.1).
+// merge (1 x 16 heads, 130 positions: 5.0 us; 8 x 16, 576: 7.9).
 // PER_SM: CTAs that an SM has to hold.  With three the kernel keeps within 168 registers, where the compiler spills a few that it
 // needs at the end; with 2 it uses 175.
 template <int HD, int NQ, bool PREFIX, int PER_SM>
@@ -997,7 +997,7 @@ __global__ void __launch_bounds__((WIDE ? kJoinWarps : kWarps) * 32) attn_flat_j
 // the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; the QW warps of a group
 // take the same tiles, which they fetch together into the group's ring, and the KW = 8 / QW groups take alternate tiles.
 // What bounds it: the s8 products of mma.sync, 8 cycles each on an SM's quarter, from 16 rows on (32 rows x 8 heads behind 16384
-// positions: 35.4 us with the decode behind it); below, start, digits and the hand-over (8 rows x 16 heads behind 2048: 11.7).
+// positions: 35.4 us with the decode behind it); below, start, digits and the hand-over (8 rows x 16 heads behind 2048: 11.4).
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
