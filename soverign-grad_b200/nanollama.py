@@ -218,7 +218,7 @@ class NanoLlamaInt4:
         self.pos = torch.zeros(1, dtype=torch.int32, device=dev)
         self._zero = torch.zeros(1, dtype=torch.int32, device=dev)
         self._bufs = {}
-        self._graph = None
+        self._graph = self._graph_ws = None              # the recorded step, and the scratch that it writes to
         self.tok = torch.zeros(batch, dtype=torch.int64, device=dev)
         self.launches_per_decode_step = 0
 
@@ -532,7 +532,7 @@ class NanoLlamaInt4:
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
             self._greedy_step()
-        self._graph = graph
+        self._graph, self._graph_ws = graph, self.ws.buf
         self.pos.copy_(saved_pos)
         self.tok.copy_(saved_tok)
         torch.cuda.synchronize()
@@ -548,7 +548,8 @@ class NanoLlamaInt4:
         self._argmax(logits)
         out[:, 0].copy_(self.tok)
         use_graph = use_graph and (self.world == 1 or self.exchange == "peer") and not keep_logits
-        if use_graph and self._graph is None:
+        # a longer prompt (or prefix) may have asked for more scratch since: a step recorded before writes to memory given back
+        if use_graph and (self._graph is None or self._graph_ws is not self.ws.buf):
             self.capture_decode_graph()
         for s in range(1, n_new):
             if use_graph:

@@ -133,6 +133,26 @@ def test_recorded_steps_are_the_eager_ones(sgq, nl, port, max_prefix, max_seq):
                 model.set_prefix(bad)
 
 
+def test_recorded_steps_leave_given_back_scratch_alone(sgq, nl, port):
+    """Batches whose linears use the scratch buffer: a long prefix makes it grow after a step has been recorded."""
+    cfg, model, _ = build(nl, port, 20, 4, max_prefix=600)
+    r = np.random.default_rng(8)
+    prompt, prefix = torch.from_numpy(r.integers(0, cfg.vocab, (20, 1))), torch.from_numpy(r.integers(0, cfg.vocab, 600))
+    model.generate(prompt, 4)
+    assert model._graph is not None
+    before, at, size = model._graph_ws, model.ws.buf.data_ptr(), model.ws.buf.numel()
+    assert before is model.ws.buf
+    del before
+    model.set_prefix(prefix)
+    assert model.ws.buf.numel() > size, "the prefix does not make the scratch grow: choose a longer one"
+    want, _ = model.generate(prompt, 9, use_graph=False, keep_logits=True)
+    model._graph_ws = None                     # what held the old scratch
+    spies = [torch.zeros(size, dtype=torch.uint8, device="cuda") for _ in range(4)]
+    assert torch.equal(model.generate(prompt, 9), want)
+    assert not any(bool(x.any()) for x in spies)
+    assert model._graph_ws is model.ws.buf and any(x.data_ptr() == at for x in spies)
+
+
 def test_a_prefix_in_front_is_the_same_tokens_in_the_prompt(sgq, nl, port):
     """The prefix's tokens once in front or in every prompt: the same definition, so every row that is held is equal up to single
     codes that fp32 noise tips over, and the logits within the fp32 tolerance of their own recompute (above); here the caches."""
