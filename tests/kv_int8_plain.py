@@ -44,8 +44,9 @@ def decode(qkv, cache, cos, sin, pos, heads, prefix=None, prefix_len=0):
     subtracted (once) and by the key's scale (once): a score is off by at most e = 8 * 2^-24 * max |q| sum |k| / sqrt(dim).
     Weights are off by 2 e (their sum as well, hence the 2), by the exponential (2 ulp: 4 * 2^-24) and by their own fixed point
     (half of 1 / 4194000 of the largest: 2 * 2^-24), 6 * 2^-24 together.  Sums over n positions round once per 32-position tile of
-    a warp, with one rescaling each, and when warps, CTAs and prefix parts are joined (at most 39 times):
-    (3 n / 256 + 39) * 2^-24 of the largest value."""
+    a warp, with one rescaling each, and when warps, CTAs and prefix parts are joined (at most 39 times; or 16 times inside
+    the tensor core, whose sums may be cut off at 2 * 2^-24, and 7 times behind it): (3 n / 256 + 39) * 2^-24 of the largest
+    value."""
     cache = {k: v.copy() for k, v in cache.items()}
     B, kv, S, dim = cache["k_codes"].shape
     G = heads // kv
