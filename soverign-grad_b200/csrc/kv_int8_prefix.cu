@@ -199,6 +199,8 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             if (x < HD / 8) cp_async_16(smem_u32(turns + i * HD + (lane >> 4) * (HD / 2) + x * 4), (lane < 16 ? a.cos_t : a.sin_t) + from + x * 4);
         }
     }
+    // A group of their own: a CTA without a tile (t0 == t1) commits no other, and a wait covers committed copies alone.
+    asm volatile("cp.async.commit_group;" ::: "memory");
 
     auto request_keys = [&](int slot, int t) {
         constexpr int CH = HD / 16;
