@@ -123,7 +123,8 @@ SGQ_API int sgqd_argmax_rows(const float* x, int64_t rows, int64_t n, int64_t ld
  * all in fp32 (a NaN gets code +127; an infinity makes the scale infinite), and stands for code * scale.  Keys are rotated
  * before they are quantized, every product and sum of the rotation rounded to fp32, so the codes depend on the inputs alone.
  * The struct holds DEVICE pointers owned by the caller; it is read during the call only.  codes: [batch, n_kv_heads,
- * max_seq, head_dim], 16-byte aligned; scales: [batch, n_kv_heads, max_seq].  Query head h reads kv head
+ * max_seq, head_dim], 16-byte aligned; scales: [batch, n_kv_heads, max_seq].  The four arrays, rows, outputs and workspace of a
+ * call share no memory (SGQ_ERR_BAD_ARGUMENT where they do), but for what is said below.  Query head h reads kv head
  * h / (n_heads / n_kv_heads).  `pos` is a DEVICE int32 per sequence (pos_stride 1) or one for all (pos_stride 0): the tokens
  * of the sequence that are in the cache.  Rows of qkv are [n_heads | n_kv_heads | n_kv_heads] heads of head_dim values,
  * qkv_stride floats apart; cos / sin tables as above, [table_rows, head_dim / 2], 16-byte aligned. */
@@ -178,7 +179,7 @@ SGQ_API int sgqd_attn_decode_int8(const float* qkv, int64_t qkv_stride, int64_t 
  * prefix->max_seq), whose rows lie once in `prefix`, a cache of one sequence with the same heads: every query attends to
  * the prefix rows and to its own rows 0 .. pos[b], which stand at positions *prefix_len + t of its sequence (the rotation of
  * the new token included; table_rows >= prefix->max_seq + max_seq).  The prefix is read once for the whole
- * batch and shares no memory with `cache`.  workspace: as for sgqd_attn_decode_int8 (0 bytes only for sizes that are refused). */
+ * batch and shares no memory with `cache` (refused).  workspace: as for sgqd_attn_decode_int8 (0 bytes only for sizes that are refused). */
 SGQ_API size_t sgqd_attn_decode_prefix_int8_workspace_bytes(int64_t batch, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
                                                             int64_t max_seq, int64_t prefix_max);
 SGQ_API int sgqd_attn_decode_prefix_int8(const float* qkv, int64_t qkv_stride, int64_t n_heads, const float* cos_table,

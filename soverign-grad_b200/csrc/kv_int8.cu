@@ -11,6 +11,7 @@
 #include <cooperative_groups.h>
 #include <math.h>
 #include <math_constants.h>
+#include <stdint.h>
 
 namespace sgq {
 
@@ -1126,12 +1127,41 @@ int check_cache_pointers(const sgqd_cache_int8* c) {
 }
 // Do `rows` rows of wx floats, sx apart, and of wy floats, sy apart, share memory?  (Columns of one wider matrix do not.)
 bool rows_overlap(const float* x, int64_t sx, int64_t wx, const float* y, int64_t sy, int64_t wy, int64_t rows) {
-    const int64_t a = static_cast<int64_t>(reinterpret_cast<uintptr_t>(x) / 4), b = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y) / 4);
-    if (a + (rows - 1) * sx + wx <= b || b + (rows - 1) * sy + wy <= a) return false;
+    using wide = __int128;
+    const wide a = reinterpret_cast<uintptr_t>(x) / 4, b = reinterpret_cast<uintptr_t>(y) / 4, steps = rows - 1;
+    if (a + steps * sx + wx <= b || b + steps * sy + wy <= a) return false;
     if (sx != sy || rows == 1) return true;
-    const int64_t d = ((b - a) % sx + sx) % sx;
+    const wide d = ((b - a) % sx + sx) % sx;
     return d < wx || d + wy > sx;
 }
+// Memory that a call reads or writes
+struct Span {
+    uintptr_t from, to;
+    bool meets(const Span& other) const { return from < other.to && other.from < to; }
+};
+Span span(const void* p, int64_t a, int64_t b, int64_t c, int64_t d) {      // a * b * c * d bytes at p, none where p is NULL
+    const uintptr_t from = reinterpret_cast<uintptr_t>(p);
+    const unsigned __int128 most = UINTPTR_MAX - from, bytes = static_cast<unsigned __int128>(a * b) * static_cast<uint64_t>(c * d);
+    return Span{from, p ? from + static_cast<uintptr_t>(std::min(bytes, most)) : from};
+}
+Span span_of_rows(const float* p, int64_t rows, int64_t stride, int64_t width) {
+    const __int128 floats = static_cast<__int128>(rows - 1) * stride + width;
+    return span(p, 1, 1, 4, static_cast<int64_t>(std::min<__int128>(floats, INT64_MAX / 4)));
+}
+struct CacheSpans {
+    Span s[4];
+    explicit CacheSpans(const sgqd_cache_int8* c)
+        : s{span(c->k_codes, c->batch, c->n_kv_heads, c->max_seq, c->head_dim), span(c->k_scales, c->batch, c->n_kv_heads, c->max_seq, 4),
+            span(c->v_codes, c->batch, c->n_kv_heads, c->max_seq, c->head_dim), span(c->v_scales, c->batch, c->n_kv_heads, c->max_seq, 4)} {}
+    bool meets(const Span& other) const { return s[0].meets(other) || s[1].meets(other) || s[2].meets(other) || s[3].meets(other); }
+    bool meets(const CacheSpans& other) const { return meets(other.s[0]) || meets(other.s[1]) || meets(other.s[2]) || meets(other.s[3]); }
+    bool apart() const {                                                    // the four arrays from one another
+        for (int i = 0; i < 4; ++i)
+            for (int j = 0; j < i; ++j)
+                if (s[i].meets(s[j])) return false;
+        return true;
+    }
+};
 CacheView view(const sgqd_cache_int8* c) { return CacheView{c->k_codes, c->k_scales, c->v_codes, c->v_scales, c->max_seq}; }
 
 // Splits of a shared prefix and rows per block of its kernel: a function of the sizes alone, so that the workspace's size is one
@@ -1315,6 +1345,17 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
     if (need && (!workspace || workspace_bytes < need || !aligned(workspace, 256)))
         return bad(SGQ_ERR_WORKSPACE, "workspace too small or not 256-byte aligned");
     if (batch * n_heads > 0x7fffff00) return bad(SGQ_ERR_BAD_SHAPE, "too many query rows for one call");
+    // The kernels run next to one another and store rows, scratch and outputs while others are still reading.
+    const CacheSpans own(cache);
+    const Span results = span_of_rows(out, batch, out_stride, n_heads * hd), rows = span_of_rows(qkv, batch, qkv_stride, (n_heads + 2 * kv) * hd),
+               scratch = span(workspace, 1, 1, 1, static_cast<int64_t>(need)),
+               planes = span(prepared_out, 1, 1, 1, prepared_out ? static_cast<int64_t>(gemv_prepared_bytes(batch, n_heads * hd)) : 0);
+    if (!own.apart()) return bad(SGQ_ERR_BAD_ARGUMENT, "the cache's arrays overlap one another");
+    if (prefix && CacheSpans(prefix).meets(own)) return bad(SGQ_ERR_BAD_ARGUMENT, "prefix and cache share memory");
+    for (const Span& written : {results, scratch, planes})
+        if (own.meets(written) || (prefix && CacheSpans(prefix).meets(written))) return bad(SGQ_ERR_BAD_ARGUMENT, "an output or the workspace overlaps a cache");
+    if (scratch.meets(results) || scratch.meets(planes) || scratch.meets(rows) || planes.meets(results) || planes.meets(rows) || own.meets(rows))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "outputs, workspace, cache and qkv overlap");
     if ((rc = check_device()) != SGQ_OK) return rc;
     DecodeArgs a = {};
     a.qkv = qkv; a.qkv_stride = qkv_stride; a.n_heads = static_cast<int>(n_heads); a.n_kv = static_cast<int>(kv); a.batch = static_cast<int>(batch);
@@ -1364,6 +1405,11 @@ int sgqd_rope_kv_store_int8(const float* qkv, int64_t qkv_stride, int64_t t_new,
         return bad(SGQ_ERR_ALIGNMENT, "rows and tables must be 16-byte aligned");
     if (q_out != qkv && rows_overlap(qkv, qkv_stride, (n_heads + 2 * kv) * hd, q_out, q_stride, n_heads * hd, cache->batch * t_new))
         return bad(SGQ_ERR_BAD_ARGUMENT, "q_out overlaps qkv and is not qkv itself");
+    const CacheSpans own(cache);
+    const int64_t tokens = cache->batch * t_new;
+    if (!own.apart()) return bad(SGQ_ERR_BAD_ARGUMENT, "the cache's arrays overlap one another");
+    if (own.meets(span_of_rows(qkv, tokens, qkv_stride, (n_heads + 2 * kv) * hd)) || own.meets(span_of_rows(q_out, tokens, q_stride, n_heads * hd)))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "the cache overlaps the rows");
     if ((rc = check_device()) != SGQ_OK) return rc;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t rows = n_heads + 2 * kv;
@@ -1408,6 +1454,12 @@ int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_t batch,
     const int64_t step = kLoadThreads / (cache->head_dim / 8), chunks = ceil_div(rows, step * kLoadRows);
     const int64_t heads = batch * cache->n_kv_heads;
     if (heads > 0x7fffffff / chunks) return bad(SGQ_ERR_BAD_SHAPE, "too many rows for one call");
+    const int64_t hd = cache->head_dim, apart = out_max_seq * hd;          // floats between the written rows of two heads
+    if (rows_overlap(k_out + out_row0 * hd, apart, rows * hd, v_out + out_row0 * hd, apart, rows * hd, heads))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "the outputs overlap");
+    const CacheSpans own(cache);
+    if (own.meets(span(k_out, heads, out_max_seq, hd, 4)) || own.meets(span(v_out, heads, out_max_seq, hd, 4)))
+        return bad(SGQ_ERR_BAD_ARGUMENT, "an output overlaps the cache");
     if ((rc = check_device()) != SGQ_OK) return rc;
     const bool wide = aligned(k_out, 32) && aligned(v_out, 32);
     SGQ_CUDA_TRY(launch_kernel(wide ? kv_load_int8_kernel<true> : kv_load_int8_kernel<false>, dim3(static_cast<unsigned>(heads * chunks), 2), dim3(kLoadThreads), 0,
