@@ -307,8 +307,8 @@ struct WarpAttention {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int h = i >> 1, r = 2 * (i & 1);
-                const float x = join_digits(acc[h][s][r], acc[h][s][r + 1], acc[h][NS][r + s]) * qu[s];
-                sc[s][i] = fmaf(x, ks[i], ks[i] - ks[i]);               // NaN for a row whose scale is not finite
+                const float x = join_digits(acc[h][s][r], acc[h][s][r + 1], acc[h][NS][r + s]) * (ks[i] * kKeyDown);
+                sc[s][i] = fmaf(x, qu[s], ks[i] - ks[i]);               // NaN for a row whose scale is not finite
             }
         if (n < kTile) {
 #pragma unroll

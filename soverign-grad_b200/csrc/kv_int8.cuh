@@ -145,12 +145,17 @@ __device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos
 // What a rotated query is multiplied with on the way to its digits, from the bits of its largest |value|, and the unit of its
 // scores, which carries 1/sqrt(HD) and log2(e).  A NaN or an infinity in the query makes the unit NaN and the digits zero: every
 // score is NaN.
+//
+// A score is (digit sum * key scale) * unit, in this order in every kernel, so that equal rows have equal scores whichever kernel
+// reads them.  Digit sums reach 2^37, key scales 2^121 and units without kKeyDown 2^102: the key scale is taken times 2^-31 and the
+// unit times 2^31, so that no factor overflows where the score is of ordinary size (queries of up to 2^122, keys of any size).
+constexpr float kKeyDown = 0x1p-31f;
 __device__ __forceinline__ bool digits_hold(uint32_t top) { return top < 0x7F800000u && __uint_as_float(top) >= 1e-30f; }
 __device__ __forceinline__ float query_scale(uint32_t top) { return digits_hold(top) ? __fdiv_rn(kDigitRange, __uint_as_float(top)) : 0.f; }
 template <int HD>
 __device__ __forceinline__ float query_unit(uint32_t top) {
     if (top >= 0x7F800000u) return CUDART_NAN_F;
-    return digits_hold(top) ? __fmul_rn(__fdiv_rn(__uint_as_float(top), kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f;
+    return digits_hold(top) ? __fmul_rn(__fdiv_rn(__uint_as_float(top), kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f * (1.0f / kKeyDown)) : 0.f;
 }
 template <int HD>
 __device__ __forceinline__ uint32_t largest_bits(const float (&v)[HD / 32]) {
@@ -159,20 +164,13 @@ __device__ __forceinline__ uint32_t largest_bits(const float (&v)[HD / 32]) {
     for (int j = 0; j < HD / 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
     return __reduce_max_sync(0xffffffffu, top);
 }
-// The rotated query as digits (at(j, d): where digit j of value d goes) and its unit
+// A query's digits, `per` being its query_scale (at(j, d): where digit j of value d goes)
 template <int HD, typename At>
-__device__ __forceinline__ void query_digits(const float (&v)[HD / 32], At at, float* unit, int lane) {
+__device__ __forceinline__ void put_digits(const float (&v)[HD / 32], float per, At at, int lane) {
     constexpr int VEC = HD / 32;
-    uint32_t top = 0;
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
-    top = __reduce_max_sync(0xffffffffu, top);
-    const float most = __uint_as_float(top);
-    const bool fine = top < 0x7F800000u && most >= 1e-30f;
-    const float per = fine ? __fdiv_rn(kDigitRange, most) : 0.f;
     uint32_t d[VEC];
 #pragma unroll
-    for (int j = 0; j < VEC; ++j) d[j] = fine ? digit_bytes(__float2int_rn(__fmul_rn(v[j], per))) : 0u;
+    for (int j = 0; j < VEC; ++j) d[j] = per != 0.f ? digit_bytes(__float2int_rn(__fmul_rn(v[j], per))) : 0u;
 #pragma unroll
     for (int j = 0; j < 3; ++j) {
         if constexpr (VEC == 4)
@@ -180,7 +178,13 @@ __device__ __forceinline__ void query_digits(const float (&v)[HD / 32], At at, f
         else
             *reinterpret_cast<uint16_t*>(at(j, lane * 2)) = static_cast<uint16_t>(__byte_perm(d[0], d[1], 0x0040 + 0x11 * j));
     }
-    if (lane == 0) *unit = top >= 0x7F800000u ? CUDART_NAN_F : (fine ? __fmul_rn(__fdiv_rn(most, kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f) : 0.f);
+}
+// The rotated query as digits and its unit
+template <int HD, typename At>
+__device__ __forceinline__ void query_digits(const float (&v)[HD / 32], At at, float* unit, int lane) {
+    const uint32_t top = largest_bits<HD>(v);
+    put_digits<HD>(v, query_scale(top), at, lane);
+    if (lane == 0) *unit = query_unit<HD>(top);
 }
 
 #endif  // __CUDACC__

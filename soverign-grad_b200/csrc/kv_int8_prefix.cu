@@ -116,21 +116,6 @@ __device__ __forceinline__ void split_weights(float2 w, uint32_t& hi, uint32_t& 
     lo = *reinterpret_cast<const uint32_t*>(&y);
 }
 
-// A query's digits as in query_digits, its scale being known
-template <int HD, typename At>
-__device__ __forceinline__ void put_digits(const float (&v)[HD / 32], float per, At at, int lane) {
-    constexpr int VEC = HD / 32;
-    uint32_t d[VEC];
-#pragma unroll
-    for (int j = 0; j < VEC; ++j) d[j] = per != 0.f ? digit_bytes(__float2int_rn(__fmul_rn(v[j], per))) : 0u;
-#pragma unroll
-    for (int j = 0; j < 3; ++j) {
-        if constexpr (VEC == 4)
-            *reinterpret_cast<uint32_t*>(at(j, lane * 4)) = gather_byte(d[0], d[1], d[2], d[3], j);
-        else
-            *reinterpret_cast<uint16_t*>(at(j, lane * 2)) = static_cast<uint16_t>(__byte_perm(d[0], d[1], 0x0040 + 0x11 * j));
-    }
-}
 // grid (kv heads, splits of the prefix, blocks of 128 rows)
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const DecodeArgs a) {
@@ -139,7 +124,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     extern __shared__ uint8_t raw[];
     uint8_t* sm = raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
     float* sm_unit = reinterpret_cast<float*>(sm + S::kSmall);
-    float* sm_ks = sm_unit + 128;                                     // [2][kTile]
+    float* sm_ks = sm_unit + 128;                                     // [2][kTile], times kKeyDown
     float* sm_vs = sm_ks + 2 * kTile;                                 // [2][kTile], relative to the tile's largest
     float* sm_lv = sm_vs + 2 * kTile;                                 // [2][kTile]: log2 of these
     float2* sm_top = reinterpret_cast<float2*>(sm_lv + 2 * kTile);    // [4][128]: a quarter's largest score, and score + sm_lv
@@ -234,7 +219,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
                 make_uint4(half2_of<0>(vr[u].x), half2_of<1>(vr[u].x), half2_of<0>(vr[u].y), half2_of<1>(vr[u].y));
         }
         // a scale that is not finite counts as NaN; positions that do not exist weigh nothing
-        if (tid < kTile) sm_ks[slot * kTile + tid] = scale + (scale - scale);
+        if (tid < kTile) sm_ks[slot * kTile + tid] = fmaf(scale, kKeyDown, scale - scale);
         else if (tid < 2 * kTile) {
             const int i = tid - kTile;
             const bool finite = scale - scale == 0.f;

@@ -90,3 +90,94 @@ def test_tensors_side_by_side_in_one_buffer(sgq):
     long = [dev(t) for t in plain.tables(2 * S, dim)]
     with pytest.raises(sgq.SgqError):
         sgq.attn_decode_prefix_int8(part[4][:1], one, one, ints(4), *long, ints(4), heads)
+
+
+# ---- near the ends of the fp32 range --------------------------------------------------------------------------------------
+# sequences, heads, kv heads, capacity and position, length of the shared prefix: a cluster of CTAs per head (4 and 8 queries), a cache dealt
+# out to all warps, and behind a prefix 4, 16, 32 and 40 query rows per kv head (8 rows per warp, one to four warps side by side; tcgen05)
+FORMS = [(2, 4, 2, 130, 99, 0), (1, 8, 1, 300, 299, 0), (1, 4, 1, 20000, 700, 0), (2, 4, 2, 40, 9, 200), (4, 8, 2, 40, 9, 200), (8, 8, 2, 40, 9, 200), (10, 8, 2, 40, 9, 200)]
+
+
+class Step:
+    """A decode step on N(0, 1) rows times q_size, k_size and v_size (the cache's, the prefix's and the new token's alike)."""
+
+    def __init__(self, form, dim, q_size, k_size, v_size, seed=0):
+        self.B, self.heads, self.kv, self.S, self.pos, self.P = form
+        self.dim = dim
+        r = np.random.default_rng(seed + dim + self.S + self.P + self.B)
+        f = lambda *shape: r.standard_normal(shape)  # noqa: E731
+        self.qkv = f(self.B, self.heads + 2 * self.kv, dim)
+        for at, size in ((slice(0, self.heads), q_size), (slice(self.heads, self.heads + self.kv), k_size), (slice(self.heads + self.kv, None), v_size)):
+            self.qkv[:, at] *= size
+        self.qkv = self.qkv.astype(np.float32)
+        self.cos, self.sin = plain.tables(self.S + self.P, dim)
+        keys, first = f(self.B, self.kv, self.S, dim) * k_size, f(1, self.kv, self.P, dim) * k_size
+        at = self.P + self.pos
+        like = plain.turned(self.qkv[:, :self.heads:self.heads // self.kv].astype(np.float64), self.cos[at], self.sin[at]) * (k_size / q_size)
+        keys[:, :, [1, self.pos - 1]] = like[:, :, None]         # keys along the first query of each kv head (of sequence 0 in the prefix), twice
+        if self.P:
+            first[0][:, [2, self.P - 1]] = like[0][:, None]
+        self.own = cache_of(keys, f(self.B, self.kv, self.S, dim) * v_size)
+        self.first = cache_of(first, f(1, self.kv, self.P, dim) * v_size) if self.P else None
+
+    def want(self):
+        return plain.decode(self.qkv.reshape(self.B, -1), self.own, self.cos, self.sin, [self.pos], self.heads, self.first, self.P)
+
+    def run(self, sgq):
+        x, cache, rest = dev(self.qkv.reshape(self.B, -1)), to_gpu(sgq, self.own), (dev(self.cos), dev(self.sin), ints(self.pos), self.heads)
+        if self.first is None:
+            return sgq.attn_decode_int8(x, cache, *rest).cpu().numpy()
+        return sgq.attn_decode_prefix_int8(x, cache, to_gpu(sgq, self.first), ints(self.P), *rest).cpu().numpy()
+
+    def check(self, sgq):
+        want, _, tol = self.want()
+        got = self.run(sgq)
+        assert np.isfinite(want).all() and np.isfinite(tol).all()
+        off = np.abs(got - want) / tol
+        assert np.isfinite(got).all() and off.max() <= 1, off.max()
+
+    def rows(self, b, h):
+        """The positions that query head h of sequence b attends to: keys and values in 64 bits, and its rotated query."""
+        hk, at = h // (self.heads // self.kv), self.P + self.pos
+        out = []
+        for name, new in (("k", plain.turned(self.qkv[b, self.heads + hk], self.cos[at], self.sin[at])), ("v", self.qkv[b, self.heads + self.kv + hk])):
+            parts = [self.first[name + "_codes"][0, hk].astype(np.float64) * self.first[name + "_scales"][0, hk, :, None]] if self.P else []
+            parts.append(self.own[name + "_codes"][b, hk, :self.pos].astype(np.float64) * self.own[name + "_scales"][b, hk, :self.pos, None])
+            codes, scale = plain.held(new)
+            parts.append(codes[None].astype(np.float64) * np.float64(scale))
+            out.append(np.concatenate(parts))
+        q = plain.turned(self.qkv[b, h].astype(np.float64), self.cos[at].astype(np.float64), self.sin[at].astype(np.float64))
+        return out[0], out[1], q
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("q_size,k_size", [(1.0, 1.0), (1.2e-30, 4e30), (1e-25, 1e25)])
+def test_large_keys_and_small_queries(sgq, form, dim, q_size, k_size):
+    """Scores of ordinary size whose factors are far from one: the bound of tests/kv_int8_plain.py, which is relative to both."""
+    Step(form, dim, q_size, k_size, 1.0).check(sgq)
+
+
+def winners(sgq, step):
+    """Where a query's largest scores are far ahead, their positions take all the weight and, having the same key, share it alike: out is
+    the mean of their values, within the weights' fixed point, their exponential, the joining of up to six and the division:
+    16 * 2^-24 of the largest.  Heads whose lead is not beyond any rounding are passed over."""
+    got = step.run(sgq).reshape(step.B, step.heads, step.dim)
+    seen = shared = 0
+    for b in range(step.B):
+        for h in range(step.heads):
+            k, v, q = step.rows(b, h)
+            s = k @ q / np.sqrt(step.dim)
+            lead = (k == k[np.argmax(s)]).all(-1)
+            room = 16 * 2.0 ** -24 * np.abs(q).max() * np.abs(k).sum(-1).max() / np.sqrt(step.dim)
+            if s.max() - s[~lead].max() > room + 100:
+                assert np.abs(got[b, h] - v[lead].mean(0)).max() <= 16 * 2.0 ** -24 * np.abs(v[lead]).max(), (b, h)
+                seen, shared = seen + 1, shared + (lead.sum() > 1)
+    assert seen > step.B * step.heads / 2 and shared >= step.kv, "choose other inputs"
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS[:-1])
+@pytest.mark.parametrize("q_size,k_size", [(1e30, 1e-3), (1.2e36, 1e-6)])
+def test_large_queries_and_small_keys(sgq, form, dim, q_size, k_size):
+    winners(sgq, Step(form, dim, q_size, k_size, 1.0))
