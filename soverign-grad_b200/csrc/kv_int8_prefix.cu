@@ -43,6 +43,9 @@ constexpr int kPlane = 128 * 128;              // an operand: 128 rows of 128 by
 constexpr int kTmemCols = 512;
 constexpr float kAhead = 6.0f;                 // see WarpAttention in kv_int8.cu
 constexpr int kWeightBits = 13;                // a row's weights reach about 2^13 before they are split: below the largest 16-bit float
+// Up to this reference a score may be a product that is not rounded: what the rounding would change, 2^-14, is what a score of an
+// fp32 evaluation is off by.  Beyond, the row's largest score has to be the reference exactly, and scores that are equal stay equal.
+constexpr float kFar = 1024.0f;
 
 template <int HD>
 struct Shape {
@@ -405,23 +408,28 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
         // The weights are taken times a power of two that brings the row's largest to about 2^13.  (Relative to the tile's largest
         // value scale alone, rows that look past this tile would keep few bits of it: beside a token that takes the weight and
         // has small values, the outputs live on weights of 2^-17.)
+        // (A far row's largest weight is not known to a power of two: the value scales count as the tile's largest.)
         const float ref = m == -CUDART_INF_F ? 0.f : m;
-        const int up = kWeightBits - __float2int_rn(fminf(fmaxf(most - ref, -100.f), 100.f));
+        const bool far = fabsf(ref) > kFar;
+        const int up = kWeightBits - __float2int_rn(fminf(fmaxf((far ? top : most) - ref, -100.f), 100.f));
         const float shifted = static_cast<float>(up) - ref;
         unit = __int_as_float((127 - up) << 23);
         float2 sum = both(0.f);
-        auto weights = [&](auto whole) {                              // whole: the tile has all its positions
+        auto weights = [&](auto plain) {                              // plain: the tile has all its positions and the warp no far row
 #pragma unroll
             for (int q = 0; q < KEYS / 8; ++q) {
                 uint32_t hi[4], lo[4];
 #pragma unroll
                 for (int y = 0; y < 4; ++y) {
                     const int x = 4 * q + y;
-                    float2 p = fma2(c[x], both(qu), both(shifted));
+                    float2 p;
+                    if constexpr (plain.value) p = fma2(c[x], both(qu), both(shifted));
+                    else p = make_float2(__fadd_rn(__fsub_rn(__fmul_rn(c[x].x, qu), ref), static_cast<float>(up)),
+                                         __fadd_rn(__fsub_rn(__fmul_rn(c[x].y, qu), ref), static_cast<float>(up)));      // (packed, ptxas fuses product and sum)
                     p.x = exp2_approx(p.x);
                     p.y = exp2_approx(p.y);
-                    if (!whole.value && KEYS * h + 2 * x >= left) p.x = 0.f;              // whatever the unit is
-                    if (!whole.value && KEYS * h + 2 * x + 1 >= left) p.y = 0.f;
+                    if (!plain.value && KEYS * h + 2 * x >= left) p.x = 0.f;              // whatever the unit is
+                    if (!plain.value && KEYS * h + 2 * x + 1 >= left) p.y = 0.f;
                     sum = add2(sum, p);
                     const float4 v4 = *reinterpret_cast<const float4*>(sm_vs + slot * kTile + KEYS * h + 2 * (x & ~1));
                     split_weights(mul2(p, y & 1 ? make_float2(v4.z, v4.w) : make_float2(v4.x, v4.y)), hi[y], lo[y]);
@@ -431,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
                 *reinterpret_cast<uint4*>(to + S::kPPlane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
             }
         };
-        if (left >= kTile) weights(std::true_type{});
+        if (left >= kTile && !__any_sync(0xffffffffu, far)) weights(std::true_type{});
         else weights(std::false_type{});
         l2 = fma2(sum, both(unit), l2);
         if (left > kTile) {

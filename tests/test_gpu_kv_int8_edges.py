@@ -177,7 +177,17 @@ def winners(sgq, step):
 
 
 @pytest.mark.parametrize("dim", [64, 128])
-@pytest.mark.parametrize("form", FORMS[:-1])
-@pytest.mark.parametrize("q_size,k_size", [(1e30, 1e-3), (1.2e36, 1e-6)])
-def test_large_queries_and_small_keys(sgq, form, dim, q_size, k_size):
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("q_size,k_size", [(1e4, 1.0), (1e15, 1e-7), (1.0, 1e12), (3e30, 1.0), (1e30, 1e-3), (1.2e36, 1e-6)])
+def test_scores_that_leave_the_largest_alone(sgq, form, dim, q_size, k_size):
+    """Among them large queries times small keys, whose scores of 1e30 are fp32 numbers."""
     winners(sgq, Step(form, dim, q_size, k_size, 1.0))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS[3:])
+@pytest.mark.parametrize("size", [20.0, 60.0, 200.0, 2000.0])
+def test_steep_scores_behind_a_prefix(sgq, form, dim, size):
+    """Largest scores of 300 to 20000: within the bound of an fp32 evaluation on both sides of the size from which the tcgen05 kernel rounds
+    them one by one."""
+    Step(form, dim, size, 1.0, 1.0).check(sgq)
