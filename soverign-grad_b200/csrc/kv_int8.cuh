@@ -150,12 +150,16 @@ __device__ __forceinline__ void rotate_row(float (&v)[HD / 32], const float* cos
 // reads them.  Digit sums reach 2^37, key scales 2^121 and units without kKeyDown 2^102: the key scale is taken times 2^-31 and the
 // unit times 2^31, so that no factor overflows where the score is of ordinary size (queries of up to 2^122, keys of any size).
 constexpr float kKeyDown = 0x1p-31f;
-__device__ __forceinline__ bool digits_hold(uint32_t top) { return top < 0x7F800000u && __uint_as_float(top) >= 1e-30f; }
-__device__ __forceinline__ float query_scale(uint32_t top) { return digits_hold(top) ? __fdiv_rn(kDigitRange, __uint_as_float(top)) : 0.f; }
+// A query below 2^-64 is lifted by 2^64 on the way, so that neither factor leaves the fp32 range however small it is.
+__device__ __forceinline__ float query_lift(uint32_t top) { return top < 0x1F800000u ? 0x1p64f : 1.0f; }
+__device__ __forceinline__ float query_scale(uint32_t top) {                 // of the lifted values
+    return top == 0u || top >= 0x7F800000u ? 0.f : __fdiv_rn(kDigitRange, __uint_as_float(top) * query_lift(top));
+}
 template <int HD>
 __device__ __forceinline__ float query_unit(uint32_t top) {
-    if (top >= 0x7F800000u) return CUDART_NAN_F;
-    return digits_hold(top) ? __fmul_rn(__fdiv_rn(__uint_as_float(top), kDigitRange), rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f * (1.0f / kKeyDown)) : 0.f;
+    if (top - 1u >= 0x7F800000u - 1u) return top == 0u ? 0.f : CUDART_NAN_F;      // rows that a block does not have: no division of zero (0.2 us)
+    const float per = rsqrtf(static_cast<float>(HD)) * 1.4426950408889634f * (1.0f / kKeyDown);
+    return __fmul_rn(__fdiv_rn(__uint_as_float(top) * query_lift(top), kDigitRange), top < 0x1F800000u ? per * 0x1p-64f : per);
 }
 template <int HD>
 __device__ __forceinline__ uint32_t largest_bits(const float (&v)[HD / 32]) {
@@ -164,7 +168,7 @@ __device__ __forceinline__ uint32_t largest_bits(const float (&v)[HD / 32]) {
     for (int j = 0; j < HD / 32; ++j) top = max(top, __float_as_uint(v[j]) & 0x7FFFFFFFu);
     return __reduce_max_sync(0xffffffffu, top);
 }
-// A query's digits, `per` being its query_scale (at(j, d): where digit j of value d goes)
+// A query's digits from its lifted values, `per` being its query_scale (at(j, d): where digit j of value d goes)
 template <int HD, typename At>
 __device__ __forceinline__ void put_digits(const float (&v)[HD / 32], float per, At at, int lane) {
     constexpr int VEC = HD / 32;
@@ -183,7 +187,10 @@ __device__ __forceinline__ void put_digits(const float (&v)[HD / 32], float per,
 template <int HD, typename At>
 __device__ __forceinline__ void query_digits(const float (&v)[HD / 32], At at, float* unit, int lane) {
     const uint32_t top = largest_bits<HD>(v);
-    put_digits<HD>(v, query_scale(top), at, lane);
+    float x[HD / 32];
+#pragma unroll
+    for (int j = 0; j < HD / 32; ++j) x[j] = v[j] * query_lift(top);
+    put_digits<HD>(x, query_scale(top), at, lane);
     if (lane == 0) *unit = query_unit<HD>(top);
 }
 

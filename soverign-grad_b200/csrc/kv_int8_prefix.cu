@@ -263,7 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
                 const uint32_t largest = largest_bits<HD>(q);
                 if (lane == i) top = largest;
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) rows[i * HD + lane * VEC + j] = q[j];
+                for (int j = 0; j < VEC; ++j) rows[i * HD + lane * VEC + j] = q[j] * query_lift(largest);
             }
         }
         const float per = query_scale(top);

@@ -152,7 +152,7 @@ class Step:
 
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("form", FORMS)
-@pytest.mark.parametrize("q_size,k_size", [(1.0, 1.0), (1.2e-30, 4e30), (1e-25, 1e25)])
+@pytest.mark.parametrize("q_size,k_size", [(1.0, 1.0), (1.2e-30, 4e30), (1e-25, 1e25), (1e-31, 1e31), (2e-34, 1e34), (1e-36, 1e36)])
 def test_large_keys_and_small_queries(sgq, form, dim, q_size, k_size):
     """Scores of ordinary size whose factors are far from one: the bound of tests/kv_int8_plain.py, which is relative to both."""
     Step(form, dim, q_size, k_size, 1.0).check(sgq)
