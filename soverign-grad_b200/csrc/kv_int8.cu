@@ -376,8 +376,9 @@ struct WarpAttention {
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) most = max_nan(most, __shfl_xor_sync(0xffffffffu, most, d));
             // weights that vanish against the reference contribute nothing; NaN and infinity make the unit NaN
-            const float per = most < 1e-30f ? 0.f : __fdividef(kWeightRange, most);
-            unit[s] = fmaf(most, 1.0f / kWeightRange, most - most);
+            const float down = most * kValueDown;                         // far below 2^126, where __fdividef ends
+            const float per = most < kVanishing ? 0.f : __fdividef(kWeightRange * kValueDown, down);
+            unit[s] = fmaf(down, 1.0f / kWeightRange, most - most);
 #pragma unroll
             for (int j = 0; j < ST; ++j) {
                 uint32_t d[4];
@@ -607,7 +608,7 @@ struct JoinedHead {
         float* to = a.out + b * a.out_stride + static_cast<int64_t>(h) * HD + lane * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float o = L == 0.f ? 0.f : A[i] / L;
+            const float o = L == 0.f ? 0.f : A[i] / L * (1.0f / kValueDown);
             to[i] = o;
             head[lane * VEC + i] = o;
         }

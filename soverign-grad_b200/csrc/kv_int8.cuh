@@ -74,6 +74,10 @@ __device__ __forceinline__ void gather_digits(const uint32_t (&d)[4], uint32_t& 
     w1 = __byte_perm(x, y, 0x7632);
     w2 = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
 }
+// Outputs are summed before they are divided by the sum of the weights, which are up to 2^6 each: they are carried times 2^-24, so
+// that values of any size hold behind 2^18 positions (and of FLT_MAX * 2^18 / n behind n).  What a tile adds is taken as nothing
+// where the largest weight times value scale is below 2^-80, with units of sums still in the fp32 range.
+constexpr float kValueDown = 0x1p-24f, kVanishing = 0x1p-80f;
 __device__ __forceinline__ float max_nan(float a, float b) {
     float r;
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));

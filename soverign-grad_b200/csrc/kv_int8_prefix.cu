@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             const float v = i < left && finite ? scale * per : 0.f;
             sm_vs[slot * kTile + i] = i < left && !finite ? CUDART_NAN_F : v;
             sm_lv[slot * kTile + i] = __log2f(fabsf(v));              // -inf where nothing is added
-            if (i == 0) sm_vunit[i_tile & 3] = top;
+            if (i == 0) sm_vunit[i_tile & 3] = top * kValueDown;
         }
     };
     if (t0 < t1) {

@@ -101,7 +101,7 @@ FORMS = [(2, 4, 2, 130, 99, 0), (1, 8, 1, 300, 299, 0), (1, 4, 1, 20000, 700, 0)
 class Step:
     """A decode step on N(0, 1) rows times q_size, k_size and v_size (the cache's, the prefix's and the new token's alike)."""
 
-    def __init__(self, form, dim, q_size, k_size, v_size, seed=0):
+    def __init__(self, form, dim, q_size, k_size, v_size, seed=0, shape_v=lambda v: v):
         self.B, self.heads, self.kv, self.S, self.pos, self.P = form
         self.dim = dim
         r = np.random.default_rng(seed + dim + self.S + self.P + self.B)
@@ -109,6 +109,7 @@ class Step:
         self.qkv = f(self.B, self.heads + 2 * self.kv, dim)
         for at, size in ((slice(0, self.heads), q_size), (slice(self.heads, self.heads + self.kv), k_size), (slice(self.heads + self.kv, None), v_size)):
             self.qkv[:, at] *= size
+        self.qkv[:, self.heads + self.kv:] = shape_v(self.qkv[:, self.heads + self.kv:])
         self.qkv = self.qkv.astype(np.float32)
         self.cos, self.sin = plain.tables(self.S + self.P, dim)
         keys, first = f(self.B, self.kv, self.S, dim) * k_size, f(1, self.kv, self.P, dim) * k_size
@@ -117,8 +118,8 @@ class Step:
         keys[:, :, [1, self.pos - 1]] = like[:, :, None]         # keys along the first query of each kv head (of sequence 0 in the prefix), twice
         if self.P:
             first[0][:, [2, self.P - 1]] = like[0][:, None]
-        self.own = cache_of(keys, f(self.B, self.kv, self.S, dim) * v_size)
-        self.first = cache_of(first, f(1, self.kv, self.P, dim) * v_size) if self.P else None
+        self.own = cache_of(keys, shape_v(f(self.B, self.kv, self.S, dim) * v_size))
+        self.first = cache_of(first, shape_v(f(1, self.kv, self.P, dim) * v_size)) if self.P else None
 
     def want(self):
         return plain.decode(self.qkv.reshape(self.B, -1), self.own, self.cos, self.sin, [self.pos], self.heads, self.first, self.P)
@@ -191,3 +192,14 @@ def test_steep_scores_behind_a_prefix(sgq, form, dim, size):
     """Largest scores of 300 to 20000: within the bound of an fp32 evaluation on both sides of the size from which the tcgen05 kernel rounds
     them one by one."""
     Step(form, dim, size, 1.0, 1.0).check(sgq)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS + [(1, 4, 1, 20000, 19999, 0), (2, 8, 4, 900, 899, 0), (33, 1, 1, 40, 9, 3000), (3, 1, 1, 40, 9, 3000)])
+@pytest.mark.parametrize("q_size", [1e-3, 1.5])
+@pytest.mark.parametrize("v_size", [1e-7, 1.0, 1e38])
+@pytest.mark.parametrize("positive", [False, True])
+def test_values_of_any_size(sgq, form, dim, q_size, v_size, positive):
+    """Up to 3e38: many of one sign, whose sum is no fp32 number, or a single one whose weight and scale are large together."""
+    shape = lambda v: np.clip(np.abs(v) if positive else v, -3e38, 3e38)  # noqa: E731
+    Step(form, dim, q_size, 1.0, v_size, shape_v=shape).check(sgq)
