@@ -608,7 +608,7 @@ struct JoinedHead {
         float* to = a.out + b * a.out_stride + static_cast<int64_t>(h) * HD + lane * VEC;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
-            const float o = L == 0.f ? 0.f : A[i] / L * (1.0f / kValueDown);
+            const float o = live ? A[i] / L * (1.0f / kValueDown) : 0.f;          // L == 0: every score is -infinity, and the output NaN
             to[i] = o;
             head[lane * VEC + i] = o;
         }

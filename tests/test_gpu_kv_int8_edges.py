@@ -203,3 +203,29 @@ def test_values_of_any_size(sgq, form, dim, q_size, v_size, positive):
     """Up to 3e38: many of one sign, whose sum is no fp32 number, or a single one whose weight and scale are large together."""
     shape = lambda v: np.clip(np.abs(v) if positive else v, -3e38, 3e38)  # noqa: E731
     Step(form, dim, q_size, 1.0, v_size, shape_v=shape).check(sgq)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+def test_scores_beyond_the_fp32_range(sgq, form, dim):
+    """Query heads 0 and 1 of the last sequence meet keys that make every score overflow, below and above; NaN, not a number that looks
+    like an output.  So does a query value beyond 2^122 (head 2).  The others are as ever."""
+    step = Step(form, dim, 1.0, 1.0, 1.0)
+    b, size = step.B - 1, np.float32(1e5)
+    along = np.ones(dim, np.float32)
+    at = step.P + step.pos
+    turn = lambda x: plain.turned(x, step.cos[at], -step.sin[at])  # noqa: E731  (rotates back)
+    for cache, i in ((step.own, b), (step.first, 0)):
+        if cache is not None:                                   # keys with a large common part: q . k is that of the part
+            keys = cache["k_codes"][i].astype(np.float32) * cache["k_scales"][i][..., None] + size
+            cache["k_codes"][i], cache["k_scales"][i] = plain.held(keys)
+    step.qkv[b, step.heads:step.heads + step.kv] = turn(along * size)
+    step.qkv[b, 0], step.qkv[b, 1] = turn(along * np.float32(-1e36)), turn(along * np.float32(1e36))
+    step.qkv[b, 2] = turn(along * np.float32(1e37))
+    want, _, tol = step.want()
+    got = step.run(sgq).reshape(step.B, step.heads, dim)
+    assert np.isnan(got[b, :3]).all()
+    fine = np.ones(got.shape, bool)
+    fine[b, :3] = False
+    off = np.abs(got - want.reshape(got.shape))
+    assert (off <= tol.reshape(got.shape))[fine].all()
