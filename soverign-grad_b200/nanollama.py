@@ -224,21 +224,25 @@ class NanoLlamaInt4:
 
     # ---- buffers -------------------------------------------------------------------------
     def _buffers(self, M: int):
-        if M not in self._bufs:
-            c, dev, W = self.cfg, self.device, self.world
-            f = lambda *s: torch.empty(*s, device=dev)  # noqa: E731
-            b = {"h": f(M, c.dim), "n": f(M, c.dim), "qkv": f(M, 3 * self.dim_local), "attn": f(M, self.dim_local),
-                 "o": f(M, c.dim // W), "gu": f(M, 2 * self.hid_local), "act": f(M, self.hid_local), "d": f(M, c.dim // W)}
-            use_prep = self.decode_path in (PATH_AUTO, PATH_GEMV)
-            for key, width in (("p_dim", c.dim), ("p_hid", c.hidden)):
-                nb = prepared_x_bytes(M, width) if use_prep else 0
-                b[key] = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
-            if W > 1:
-                b["p_hid"] = None          # the SiLU gate output is a column slice per rank: converted after the gather
-                b.update({"g_attn": f(W, M, self.dim_local), "g_o": f(W, M, c.dim // W), "g_act": f(W, M, self.hid_local),
-                          "attn_full": f(M, c.dim), "o_full": f(M, c.dim), "act_full": f(M, c.hidden), "d_full": f(M, c.dim)})
+        """Activations of a pass over M rows.  The decode-sized ones are kept, recorded steps hold their addresses; those of a prompt
+        or a prefix go with their pass, so that lengths that come once leave nothing behind."""
+        if M in self._bufs:
+            return self._bufs[M]
+        c, dev, W = self.cfg, self.device, self.world
+        f = lambda *s: torch.empty(*s, device=dev)  # noqa: E731
+        b = {"h": f(M, c.dim), "n": f(M, c.dim), "qkv": f(M, 3 * self.dim_local), "attn": f(M, self.dim_local),
+             "o": f(M, c.dim // W), "gu": f(M, 2 * self.hid_local), "act": f(M, self.hid_local), "d": f(M, c.dim // W)}
+        use_prep = self.decode_path in (PATH_AUTO, PATH_GEMV)
+        for key, width in (("p_dim", c.dim), ("p_hid", c.hidden)):
+            nb = prepared_x_bytes(M, width) if use_prep else 0
+            b[key] = torch.empty(nb, dtype=torch.uint8, device=dev) if nb else None
+        if W > 1:
+            b["p_hid"] = None          # the SiLU gate output is a column slice per rank: converted after the gather
+            b.update({"g_attn": f(W, M, self.dim_local), "g_o": f(W, M, c.dim // W), "g_act": f(W, M, self.hid_local),
+                      "attn_full": f(M, c.dim), "o_full": f(M, c.dim), "act_full": f(M, c.hidden), "d_full": f(M, c.dim)})
+        if M == self.batch:
             self._bufs[M] = b
-        return self._bufs[M]
+        return b
 
     def _peer(self, M: int):
         """The symmetric buffers, if this pass exchanges through peer stores: the decode steps of a sharded model,
