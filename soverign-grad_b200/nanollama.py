@@ -552,7 +552,8 @@ class NanoLlamaInt4:
         self._argmax(logits)
         out[:, 0].copy_(self.tok)
         use_graph = use_graph and (self.world == 1 or self.exchange == "peer") and not keep_logits
-        # a longer prompt (or prefix) may have asked for more scratch since: a step recorded before writes to memory given back
+        # A longer prompt (or prefix) may have asked for more scratch since.  A step recorded before goes on using the buffer that it was
+        # recorded with, which _graph_ws keeps alive; recording it again gives that one back.
         if use_graph and (self._graph is None or self._graph_ws is not self.ws.buf):
             self.capture_decode_graph()
         for s in range(1, n_new):

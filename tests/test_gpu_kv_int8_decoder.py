@@ -53,3 +53,27 @@ def test_passes_of_other_sizes_leave_a_recorded_step_alone(sgq):
         for p, w in zip(prompts, want):
             model.set_prefix(prefix)
             assert torch.equal(model.generate(p, 6), w)
+
+
+def test_a_step_is_recorded_again_when_the_scratch_has_grown_and_only_then(sgq):
+    """Batches whose linears use the scratch buffer.  Nothing but the model itself touches what generate goes by."""
+    cfg, model = decoder(sgq, 20, max_prefix=600)
+    r = np.random.default_rng(4)
+    tokens = lambda *s: torch.from_numpy(r.integers(0, cfg.vocab, s))  # noqa: E731
+    prompt = tokens(20, 1)
+    model.generate(prompt, 4)
+    step, scratch = model._graph, model.ws.buf
+    assert step is not None and model._graph_ws is scratch
+    model.set_prefix(tokens(5))
+    model.generate(prompt, 4)
+    assert model.ws.buf is scratch, "so short a prefix makes the scratch grow: choose a shorter one"
+    assert model._graph is step and model._graph_ws is scratch
+    model.set_prefix(tokens(600))
+    assert model.ws.buf is not scratch, "the prefix does not make the scratch grow: choose a longer one"
+    assert model._graph is step and model._graph_ws is scratch           # kept alive as long as the step is
+    want, _ = model.generate(prompt, 9, use_graph=False, keep_logits=True)
+    assert model._graph is step
+    assert torch.equal(model.generate(prompt, 9), want)
+    assert model._graph is not step and model._graph_ws is model.ws.buf
+    step = model._graph
+    assert torch.equal(model.generate(prompt, 9), want) and model._graph is step
