@@ -229,3 +229,60 @@ def test_scores_beyond_the_fp32_range(sgq, form, dim):
     fine[b, :3] = False
     off = np.abs(got - want.reshape(got.shape))
     assert (off <= tol.reshape(got.shape))[fine].all()
+
+
+# ---- every row, once ------------------------------------------------------------------------------------------------------
+# sequences, heads, kv heads, capacity, positions, length and capacity of the prefix
+ROWS = [(8, 16, 16, 640, [575], 0, 0), (1, 16, 16, 9000, [8999], 0, 0), (2, 16, 2, 9000, [8999, 4500], 0, 0), (40, 32, 32, 600, [599], 0, 0),
+        (33, 8, 8, 1500, [1499], 0, 0), (1, 4, 1, 40000, [39999], 0, 0), (5, 10, 2, 700, [699, 64, -1, 127, 0], 0, 0),
+        (1, 4, 2, 80000, [70001], 0, 0), (4, 32, 8, 4096, [4095, 1, 63, 2049], 0, 0), (2, 32, 4, 30000, [29999, 127], 0, 0),
+        (6, 6, 6, 7000, [6999, -1, 64, 128, -1, 3500], 0, 0), (30, 4, 1, 3000, [100 * i - 1 for i in range(30)], 0, 0),
+        (2, 4, 2, 40, [33, 2], 20011, 20480), (4, 12, 4, 40, [33, 0, 39, -1], 4999, 5000), (7, 4, 1, 40, [33], 9001, 9100),
+        (12, 4, 1, 40, [33], 20011, 20480), (50, 4, 1, 40, [20], 5000, 5000), (35, 16, 8, 300, [299], 1025, 4000), (10, 40, 10, 12, [11], 129, 129),
+        (16, 16, 16, 64, [63], 777, 800), (3, 6, 6, 7000, [6999, 5, 100], 700, 720)]
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("B,heads,kv,S,pos,P,room", ROWS)
+def test_every_row_counts_once(sgq, B, heads, kv, S, pos, P, room, dim):
+    """Keys of zero: all n positions weigh 1 / n.  Row t holds one value, 127 s_t in column t mod dim with s_t between 0.5 and 1, so a row that is
+    missed, or read twice, changes its column by s_t of the sum of about n / dim such, relative to what stands there.
+
+    All terms are positive, so errors are relative too: 24 * 2^-24 for a term (the weight's fixed point, half a step of 1 / 4194000 of the
+    largest, which is at most twice the term: 4; its exponential and the division for its unit, 2 ulp each: 8; products, conversions
+    and the final division: the rest), and 2^-24 for each addition in a row, of outputs and of weights.  A warp takes every fourth step of at
+    least 32 positions or less (128 positions a step in the tcgen05 kernel), so that n / 128 + 1 additions follow one another, and 40 join parts."""
+    r = np.random.default_rng(S + P + B + dim)
+
+    def rows(batch, n, first):
+        codes, scales = np.zeros((batch, kv, n, dim), np.int8), r.uniform(0.5, 1.0, (batch, kv, n)).astype(np.float32)
+        codes[:, :, np.arange(n), (first + np.arange(n)) % dim] = 127
+        return {"k_codes": np.zeros_like(codes), "k_scales": np.ones_like(scales), "v_codes": codes, "v_scales": scales}
+
+    own, first = rows(B, S, P), rows(1, room, 0) if room else None
+    each = pos if len(pos) > 1 else pos * B
+    qkv = np.zeros((B, heads + 2 * kv, dim), np.float32)
+    qkv[:, :heads] = r.standard_normal((B, heads, dim))
+    for b, p in enumerate(each):
+        if p >= 0:
+            qkv[b, heads + kv:, (P + p) % dim] = r.uniform(63, 127, kv)
+    cos, sin = plain.tables(S + room, dim)
+    args = (dev(qkv.reshape(B, -1)), to_gpu(sgq, own))
+    rest = (dev(cos), dev(sin), ints(*pos), heads)
+    got = sgq.attn_decode_prefix_int8(*args, to_gpu(sgq, first), ints(P), *rest) if room else sgq.attn_decode_int8(*args, *rest)
+    got = got.cpu().numpy().reshape(B, kv, heads // kv, dim)
+    for b, p in enumerate(each):
+        if p < 0:
+            assert not got[b].any()
+            continue
+        n = P + p + 1
+        tol = (24 + 2 * (n / 128 + 1 + 40)) * 2.0 ** -24
+        for h in range(kv):
+            sizes = [first["v_scales"][0, h, :P].astype(np.float64)] if P else []
+            codes, scale = plain.held(qkv[b, heads + kv + h])
+            assert codes[(P + p) % dim] == 127
+            sizes = 127 * np.concatenate(sizes + [own["v_scales"][b, h, :p].astype(np.float64), [np.float64(scale)]])
+            total = np.bincount(np.arange(n) % dim, sizes, dim)
+            assert (sizes / total[np.arange(n) % dim]).min() > 4 * tol, "a lost row would not show"
+            off = np.abs(got[b, h] - total / n)
+            assert (off <= tol * total / n).all(), (b, h, (off / np.maximum(total / n, 1e-30)).max() / tol, np.nonzero((off > tol * total / n).any(0))[0][:8])
