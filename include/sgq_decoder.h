@@ -160,13 +160,17 @@ SGQ_API int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_
  * its value to the cache, quantized as above, and writes
  *   out[b, h*head_dim + d] = sum_{t <= pos[b]} softmax_t(q_h . k_t / sqrt(head_dim)) v_t[d],
  * k_t and v_t being the values the cache then holds, the new token's included.  qkv is read only.  A sequence whose pos lies
- * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  A NaN or an infinity in a query
- * gives NaN in its head's output, and so does a row with a scale that is not finite, a rotated query value beyond 2^122
- * or a largest score beyond the fp32 range on either side (keys may have any size; values too behind 2^18 positions, and up to
- * FLT_MAX * 2^18 / n behind n; positions whose weight times value scale is below 2^-80 may count as nothing); rows at positions behind pos are not
- * read.  The query enters exact integer products as 24-bit fixed point relative to its largest value, the softmax weights
- * as 23-bit fixed point relative to the largest of 32 to 128 positions (behind a prefix also as the sum of two 16-bit
- * floats, 22 bits), sums are fp32: errors are those of an fp32 evaluation.  table_rows >= max_seq.  head_dim must be 64 or
+ * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  Rows at positions behind pos are not
+ * read.
+ *   Range: a NaN or an infinity in a query gives NaN in its head's output, and so does a row with a scale that is not finite, a
+ * rotated query value beyond 2^122 or a largest score beyond the fp32 range on either side.  Keys may have any size; values too behind
+ * 2^18 positions, and up to FLT_MAX * 2^18 / n behind n; positions whose weight times value scale is below 2^-80 may count as nothing.
+ *   Errors: scores are exact integer products of the codes with the query as 24-bit fixed point relative to the largest |value| of its row,
+ * off by at most 2^-21 * max |q| * sum |k_t| / sqrt(head_dim).  That is an fp32 evaluation's error where the query's values are of one
+ * order; where one is far larger than the others and its keys are small, it is larger than that by as much.  Softmax weights (times
+ * value scale) are 23-bit fixed point relative to the largest of the 32 to 128 positions that are read together (for 33 query rows and
+ * more per kv head behind a prefix the sum of two 16-bit floats, 22 bits of a weight and 2^-37 of the largest).  Exponentials are off
+ * by 2 ulp; sums are fp32.  table_rows >= max_seq.  head_dim must be 64 or
  * 128, max_seq at most 2^30.  out may not overlap qkv.  prepared_out: as for sgqd_attn_decode.  workspace: as many bytes as the query says (0: none is read; caches that
  * may grow long need some), 256-byte aligned; it holds nothing from one call to the next, and calls that may run at the
  * same time need one each.  The query's answer follows from the sizes alone. */

@@ -145,7 +145,10 @@ __global__ void __launch_bounds__(kLoadThreads) kv_load_int8_kernel(const int8_t
 // ---- decode attention -------------------------------------------------------------------------------------------------
 // Both products of the attention run on the tensor cores as exact integer products (mma.sync m16n8k32, s8 x s8 -> s32): the
 // codes go in as they lie in memory, the query and the softmax weights as 24-bit fixed point split into three balanced
-// base-256 digits (the arithmetic of gemv_prepare.cuh), one digit per column of the small operand.
+// base-256 digits (the arithmetic of gemv_prepare.cuh), one digit per column of the small operand.  A query has one scale, that of its
+// largest value: a value far below it keeps as many bits less.  (Scales per 32 values, as the linears have, would end the integer
+// sums, and the conversions behind them, four times as often; a fourth digit would take eight queries a fourth column set and the
+// tcgen05 kernel more columns than tensor memory has.)
 //
 //   scores   A = 16 rows of the cache x 32 values, B = 32 values x 8 columns.  A lane (g, t) = (lane / 4, lane % 4) of the
 //            warp reads the 16-byte chunks t (and 4 + t) of the rows 4g .. 4g+3 of a tile of 32 positions: these ARE the A

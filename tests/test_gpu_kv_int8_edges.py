@@ -286,3 +286,35 @@ def test_every_row_counts_once(sgq, B, heads, kv, S, pos, P, room, dim):
             assert (sizes / total[np.arange(n) % dim]).min() > 4 * tol, "a lost row would not show"
             off = np.abs(got[b, h] - total / n)
             assert (off <= tol * total / n).all(), (b, h, (off / np.maximum(total / n, 1e-30)).max() / tol, np.nonzero((off > tol * total / n).any(0))[0][:8])
+
+
+# ---- one value of a query far above the others ----------------------------------------------------------------------------
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("times", [30, 300, 3000])
+def test_queries_with_one_large_value(sgq, form, dim, times):
+    """A rotary pair of the queries `times` the others, its keys as much smaller, so that it adds to the scores what any other does.  The bound
+    that the header states holds: the query's fixed point is relative to its largest value, so the score's error is too
+    (tests/kv_int8_plain.py has it with max |q|), and the error is not merely that of an fp32 evaluation."""
+    step = Step(form, dim, 1.0, 1.0, 1.0)
+    pair = [5, 5 + dim // 2]
+    step.qkv[:, :step.heads, pair] *= times
+    step.qkv[:, step.heads:step.heads + step.kv, pair] /= times
+    for cache in (step.own, step.first):
+        if cache is not None:
+            keys = cache["k_codes"].astype(np.float32) * cache["k_scales"][..., None]
+            keys[..., pair] /= times
+            cache["k_codes"], cache["k_scales"] = plain.held(keys)
+    step.check(sgq)
+    got = step.run(sgq).reshape(step.B, step.heads, dim)
+    for b in range(step.B):                     # the same, per head and with what a score is made of in the place of the largest sum of all
+        for h in range(step.heads):
+            k, v, q = step.rows(b, h)
+            e = 2.0 ** -21 * np.abs(q).max() * np.abs(k).sum(-1) / np.sqrt(dim)
+            s = k @ q / np.sqrt(dim)
+            w = np.exp(s - s.max())
+            w /= w.sum()
+            want = w @ v
+            # d out = sum w (v - out) ds, and the second order of ds; 45 + 3 n / 32 roundings of weights and sums as everywhere
+            room = (w * e) @ np.abs(v - want) * (1 + 2 * e.max()) + np.abs(v).max() * (45 + 3 * len(s) / 32) * 2.0 ** -24
+            assert (np.abs(got[b, h] - want) <= room).all(), (b, h)
