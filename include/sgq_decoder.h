@@ -160,8 +160,8 @@ SGQ_API int sgqd_kv_load_int8(const sgqd_cache_int8* cache, int64_t rows, int64_
  * its value to the cache, quantized as above, and writes
  *   out[b, h*head_dim + d] = sum_{t <= pos[b]} softmax_t(q_h . k_t / sqrt(head_dim)) v_t[d],
  * k_t and v_t being the values the cache then holds, the new token's included.  qkv is read only.  A sequence whose pos lies
- * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  Rows at positions behind pos are not
- * read.
+ * outside [0, max_seq) takes no part: nothing is stored and its output row is zero.  Rows at positions behind pos may be read, as far as
+ * max_seq, but do not enter: they may hold anything, and another stream may write them meanwhile.
  *   Range: a NaN or an infinity in a query gives NaN in its head's output, and so does a row with a scale that is not finite, a
  * rotated query value beyond 2^122 or a largest score beyond the fp32 range on either side.  Keys may have any size; values too behind
  * 2^18 positions, and up to FLT_MAX * 2^18 / n behind n; positions whose weight times value scale is below 2^-80 may count as nothing.

@@ -318,3 +318,22 @@ def test_queries_with_one_large_value(sgq, form, dim, times):
             # d out = sum w (v - out) ds, and the second order of ds; 45 + 3 n / 32 roundings of weights and sums as everywhere
             room = (w * e) @ np.abs(v - want) * (1 + 2 * e.max()) + np.abs(v).max() * (45 + 3 * len(s) / 32) * 2.0 ** -24
             assert (np.abs(got[b, h] - want) <= room).all(), (b, h)
+
+
+def test_rows_behind_the_position_may_change_meanwhile(sgq):
+    """Caches of which a few positions are in use, while another stream writes all the rows behind them over and over."""
+    r = np.random.default_rng(6)
+    for B, heads, kv, S, pos in ((8, 16, 16, 640, 129), (2, 16, 2, 9000, 40), (1, 8, 2, 80000, 600)):
+        host = cache_of(r.standard_normal((B, kv, S, 128)), r.standard_normal((B, kv, S, 128)))
+        cache, x = to_gpu(sgq, host), dev(r.standard_normal((B, (heads + 2 * kv) * 128)).astype(np.float32))
+        cos, sin = (dev(t) for t in plain.tables(S, 128))
+        at, side = ints(pos), torch.cuda.Stream()
+        want = sgq.attn_decode_int8(x, cache, cos, sin, at, heads)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            for i in range(60):
+                for t, value in ((cache.k_codes, -128), (cache.k_scales, float("nan")), (cache.v_codes, i), (cache.v_scales, float("inf"))):
+                    t[:, :, pos + 1:].fill_(value)
+        got = [sgq.attn_decode_int8(x, cache, cos, sin, at, heads) for _ in range(100)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)
