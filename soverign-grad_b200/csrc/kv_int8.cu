@@ -191,15 +191,9 @@ struct Half {
     template <bool KEYS>
     static __device__ __forceinline__ int at(int row, int chunk) { return KEYS ? key_at(row, chunk) : value_at(row, chunk); }
 };
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // `THREADS` threads (this one is number i) ask for the rows codes[t ..] and their scales; rows from t1 on repeat the last one
 // (their positions are masked).
@@ -244,7 +238,6 @@ struct WarpAttention {
     static constexpr int VW = VB / 4;
     static constexpr int NS = NQ / 4, NT = NS + 1;
     static constexpr int kQueryBytes = 3 * HD; // digit planes of one query: [digit][HD]
-    static constexpr float kAhead = 6.0f;
 
     const uint8_t* planes;                     // the queries' digits, in shared memory
     float qu[NS], m[NS], l[NS], o[NS][VB];
@@ -587,15 +580,6 @@ struct JoinedHead {
             M = mn;
         }
     }
-    static __device__ __forceinline__ void load(const float* from, float (&v)[VEC]) {
-        if constexpr (VEC == 4) {
-            const float4 x = *reinterpret_cast<const float4*>(from);
-            v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-        } else {
-            const float2 x = *reinterpret_cast<const float2*>(from);
-            v[0] = x.x; v[1] = x.y;
-        }
-    }
     // joins the prefix's partial results, divides, stores query head h of sequence b (`head`: HD floats of shared memory)
     template <bool PREFIX>
     __device__ __forceinline__ void finish(const DecodeArgs& a, int b, int h, bool live, float* head, int lane) {
@@ -605,7 +589,7 @@ struct JoinedHead {
             join<6>(a.parts, [&](int p, float& m, float& l, float (&v)[VEC]) {
                 m = a.part_ml[2 * (p0 + p)];
                 l = a.part_ml[2 * (p0 + p) + 1];
-                load(a.part_o + (p0 + p) * HD + lane * VEC, v);
+                load_values_of(a.part_o + (p0 + p) * HD + lane * VEC, v);
             });
         }
         float* to = a.out + b * a.out_stride + static_cast<int64_t>(h) * HD + lane * VEC;
@@ -771,7 +755,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
         j.template join<4>(S, [&](int r, float& m, float& l, float (&v)[VEC]) {
             m = sm_part_ml[2 * (i * S + r)];
             l = sm_part_ml[2 * (i * S + r) + 1];
-            JoinedHead<HD>::load(sm_part + (i * S + r) * HD + lane * VEC, v);
+            load_values_of(sm_part + (i * S + r) * HD + lane * VEC, v);
         });
         j.template finish<PREFIX>(a, b, hk * G + q0 + split + i * S, live, sm_o + warp * HD, lane);
     }
@@ -979,7 +963,7 @@ __global__ void __launch_bounds__((WIDE ? kJoinWarps : kWarps) * 32) attn_flat_j
         const int64_t at = (unit + w_first + p * BY) * NQ + g % NQ;
         m = a.flat_ml[2 * at];
         l = a.flat_ml[2 * at + 1];
-        JoinedHead<HD>::load(a.flat_o + at * HD + lane * VEC, v);
+        load_values_of(a.flat_o + at * HD + lane * VEC, v);
     });
     if constexpr (WIDE) {
         if (lane == 0) { sm_ml[warp][0] = t.M; sm_ml[warp][1] = t.L; }
@@ -991,7 +975,7 @@ __global__ void __launch_bounds__((WIDE ? kJoinWarps : kWarps) * 32) attn_flat_j
         t.template join<4>(W, [&](int u, float& m, float& l, float (&v)[VEC]) {
             m = sm_ml[u][0];
             l = sm_ml[u][1];
-            JoinedHead<HD>::load(&sm_o[u][lane * VEC], v);
+            load_values_of(&sm_o[u][lane * VEC], v);
         });
         __syncwarp();
     }

@@ -74,6 +74,8 @@ __device__ __forceinline__ void gather_digits(const uint32_t (&d)[4], uint32_t& 
     w1 = __byte_perm(x, y, 0x7632);
     w2 = __byte_perm(__byte_perm(d[0], d[1], 0x0062), __byte_perm(d[2], d[3], 0x0062), 0x5410);
 }
+// The reference that weights are taken against follows the maximum only when a score exceeds it by kAhead: weights of up to 2^kAhead.
+constexpr float kAhead = 6.0f;
 // Outputs are summed before they are divided by the sum of the weights, which are up to 2^6 each: they are carried times 2^-24, so
 // that values of any size hold behind 2^18 positions (and of FLT_MAX * 2^18 / n behind n).  What a tile adds is taken as nothing
 // where the largest weight times value scale is below 2^-80, with units of sums still in the fp32 range.
@@ -88,6 +90,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // N = 4 or 8 consecutive floats, aligned to their own size
 template <int N>
@@ -109,6 +118,19 @@ __device__ __forceinline__ void store_floats(float* p, const float (&v)[N]) {
                      "f"(v[6]), "f"(v[7])
                      : "memory");
     else *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+}
+
+// A lane's HD / 32 consecutive values of a row
+template <int N>
+__device__ __forceinline__ void load_values_of(const float* from, float (&v)[N]) {
+    static_assert(N == 2 || N == 4, "head sizes of 64 and 128");
+    if constexpr (N == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(from);
+        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    } else {
+        const float2 x = *reinterpret_cast<const float2*>(from);
+        v[0] = x.x; v[1] = x.y;
+    }
 }
 
 // Joins partial results (maximum, sum, value) of one output value

@@ -41,7 +41,6 @@ namespace {
 constexpr int kThreads = 512, kRows = kPrefixTcRows, kTile = kPrefixTcTile;
 constexpr int kPlane = 128 * 128;              // an operand: 128 rows of 128 bytes
 constexpr int kTmemCols = 512;
-constexpr float kAhead = 6.0f;                 // see WarpAttention in kv_int8.cu
 constexpr int kWeightBits = 13;                // a row's weights reach about 2^13 before they are split: below the largest 16-bit float
 // Up to this reference a score may be a product that is not rounded: what the rounding would change, 2^-14, is what a score of an
 // fp32 evaluation is off by.  Beyond, the row's largest score has to be the reference exactly, and scores that are equal stay equal.
@@ -59,22 +58,6 @@ struct Shape {
 
 // 16-byte chunk c of row r of a 128-byte-swizzled operand
 __device__ __forceinline__ int swizzled(int r, int c) { return r * 128 + ((c ^ (r & 7)) << 4); }
-
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-
-template <int N>
-__device__ __forceinline__ void load_values_of(const float* from, float (&v)[N]) {
-    static_assert(N == 2 || N == 4, "head sizes of 64 and 128");
-    if constexpr (N == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(from);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-    } else {
-        const float2 x = *reinterpret_cast<const float2*>(from);
-        v[0] = x.x; v[1] = x.y;
-    }
-}
 
 // Two fp32 operations in one instruction
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
@@ -188,7 +171,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
         }
     }
     // A group of their own: a CTA without a tile (t0 == t1) commits no other, and a wait covers committed copies alone.
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    cp_async_commit();
 
     auto request_keys = [&](int slot, int t) {
         constexpr int CH = HD / 16;
@@ -197,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
             const int x = tid + u * kThreads, r = x / CH, c = x % CH;
             cp_async_16(sm_u + S::kK + slot * kPlane + swizzled(r, c), kc + static_cast<int64_t>(t) * HD + min(r, t1 - 1 - t) * HD + c * 16);
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+        cp_async_commit();
     };
     // values: 8 codes of a row per load, which are a 16-byte chunk of the operand
     constexpr int VCH = HD / 8, VN = kTile * VCH / kThreads;
@@ -244,7 +227,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
     // Queries: every warp turns eight raw rows, which lie where the weights will, with cosines and sines where the values will, into
     // digits, four at a time.  (All unrolled with everything in registers this took 12000 cycles, most of them for code.)
     {
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        cp_async_wait<0>();
         __syncwarp();
         uint32_t top = 0;                                             // lane i: the largest of row i
 #pragma unroll 1
@@ -377,7 +360,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
         top *= qu;
         sm_top[h * kRows + row] = make_float2(top, most);
         if (!fine) *gave_up = 1;
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        cp_async_wait<0>();
         fence_proxy_async_smem();
         tcgen05_fence_before();
         __syncthreads();                                              // the scores have been read, the next keys are there
@@ -463,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, 1) attn_prefix_tc_int8_kernel(const 
         atomicCAS(&g_status_kv, 0u, (static_cast<uint32_t>(kDevErrMmaWait) << 24) | 1u);
         for (int i = 0; i < 1000; ++i) __nanosleep(1000);
     }
-    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    cp_async_wait<0>();
     const float l = l2.x + l2.y;
     float* sm_sum = reinterpret_cast<float*>(sm_top);                // [4][128]
     sm_sum[h * kRows + row] = l;
