@@ -1319,6 +1319,7 @@ int attn_decode(const float* qkv, int64_t qkv_stride, int64_t n_heads, const flo
     if ((rc = check_cache_pointers(cache)) != SGQ_OK || (prefix && (rc = check_cache_pointers(prefix)) != SGQ_OK)) return rc;
     if (!aligned(qkv, 16) || (qkv_stride & 3) || !aligned(cos_table, 16) || !aligned(sin_table, 16))
         return bad(SGQ_ERR_ALIGNMENT, "qkv rows and tables must be 16-byte aligned");
+    if (!aligned(pos, 4) || !aligned(out, 4) || !aligned(prefix_len, 4)) return bad(SGQ_ERR_ALIGNMENT, "pos, prefix_len and out must be 4-byte aligned");
     if (rows_overlap(qkv, qkv_stride, (n_heads + 2 * kv) * hd, out, out_stride, n_heads * hd, batch))
         return bad(SGQ_ERR_BAD_ARGUMENT, "out overlaps qkv");
     PreparedLayout L = {};
@@ -1391,6 +1392,7 @@ int sgqd_rope_kv_store_int8(const float* qkv, int64_t qkv_stride, int64_t t_new,
     if ((rc = check_cache_pointers(cache)) != SGQ_OK) return rc;
     if (!aligned(qkv, 16) || (qkv_stride & 3) || !aligned(q_out, 16) || (q_stride & 3) || !aligned(cos_table, 16) || !aligned(sin_table, 16))
         return bad(SGQ_ERR_ALIGNMENT, "rows and tables must be 16-byte aligned");
+    if (!aligned(pos, 4) || !aligned(n_new, 4) || !aligned(rope_offset, 4)) return bad(SGQ_ERR_ALIGNMENT, "pos, n_new and rope_offset must be 4-byte aligned");
     if (q_out != qkv && rows_overlap(qkv, qkv_stride, (n_heads + 2 * kv) * hd, q_out, q_stride, n_heads * hd, cache->batch * t_new))
         return bad(SGQ_ERR_BAD_ARGUMENT, "q_out overlaps qkv and is not qkv itself");
     const CacheSpans own(cache);

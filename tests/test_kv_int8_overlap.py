@@ -1,5 +1,5 @@
-"""Calls of the INT8 key/value cache whose tensors share memory that one of them writes: refused before a device is touched.  Every
-call here overlaps; what does not would be launched on these made-up addresses."""
+"""Calls of the INT8 key/value cache whose tensors share memory that one of them writes, or that lie off the grid of their type: refused
+before a device is touched.  Every call here is one; any other would be launched on these made-up addresses."""
 import ctypes as C
 
 import pytest
@@ -14,7 +14,7 @@ def sgq():
 B, HEADS, KV, DIM, S, P = 2, 4, 2, 128, 16, 32
 CODES, SCALES = B * KV * S * DIM, B * KV * S * 4
 AT = {name: (i + 1) << 24 for i, name in enumerate(("k", "ks", "v", "vs", "pk", "pks", "pv", "pvs", "qkv", "out", "planes", "ws", "tables", "v_out"))}
-BAD_ARGUMENT = 3
+BAD_ARGUMENT, ALIGNMENT = 3, 6
 
 
 def ptr(x):
@@ -89,3 +89,14 @@ def test_load_into_one_tensor_twice(sgq, k, v, rows, room, row0):
 def test_load_over_the_cache(sgq, name, size):
     assert sgq.lib.sgqd_kv_load_int8(own(sgq, AT), S, B, ptr(AT[name] + size - 64), ptr(AT["v_out"]), S, 0, None) == BAD_ARGUMENT
     assert sgq.lib.sgqd_kv_load_int8(own(sgq, AT), S, B, ptr(AT["v_out"]), ptr(AT[name]), S, 0, None) == BAD_ARGUMENT
+
+
+@pytest.mark.parametrize("off", [1, 2, 3])
+def test_small_vectors_off_their_grid(sgq, off):
+    p, t, q = ptr(AT["tables"] + off), ptr(AT["tables"]), ptr(AT["qkv"])
+    for pos, n_new, offset in ((p, None, None), (t, p, None), (t, None, p)):
+        assert sgq.lib.sgqd_rope_kv_store_int8(q, 1024, 1, HEADS, t, t, S, pos, 1, n_new, offset, ptr(AT["out"]), 512, own(sgq, AT), None) == ALIGNMENT
+    for pos, out in ((p, ptr(AT["out"])), (t, ptr(AT["out"] + off))):
+        assert sgq.lib.sgqd_attn_decode_int8(q, 1024, HEADS, t, t, S, pos, 1, own(sgq, AT), out, 512, None, 0, None, 0, None) == ALIGNMENT
+    assert sgq.lib.sgqd_attn_decode_prefix_int8(q, 1024, HEADS, t, t, S + P, t, 1, own(sgq, AT), first(sgq, AT), p, ptr(AT["out"]), 512, None, 0,
+                                                ptr(AT["ws"]), 1 << 20, None) == ALIGNMENT
