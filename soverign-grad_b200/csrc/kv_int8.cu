@@ -625,9 +625,10 @@ struct DecodeShape {
     static constexpr int kNew = (kSmall + (NQ + 2 * kRecv + 2 * kDecodeWarps * NQ) * 4 + 15) / 16 * 16;
     static constexpr int kBytes = kNew + NewRows<HD>::kBytes;
 };
-// What bounds it: bytes where caches are long (32 x 8 kv heads x 4 queries, up to 8192 positions, 287 MB: 54.3 us, 0.81 of the rate of
-// a plain copy; all of 4096: 49.8, 0.85), a chain of latencies where they are short: position, cosines, digits, first tile,
-// merge (1 x 16 heads, 130 positions: 5.0 us; 8 x 16, 576: 7.9).
+// What bounds it: bytes where caches are long (32 x 8 kv heads x 4 queries, up to 8192 positions, 287 MB: 53.8 to 57.1 us from box to box, 0.77
+// to 0.81 of the rate of a plain copy; all of 4096: 49.4, 0.86), a chain of latencies where they are short: position, cosines,
+// digits, first tile, merge (1 x 16 heads, 130 positions: 5.1 us; 8 x 16, 576: 7.9).  Groups of more than eight queries read the rows once for
+// every eight (32 x 8 kv heads, 4096 positions: 57.5 us with 8 queries, 104 with 16, 184 with 32).
 // PER_SM: CTAs that an SM has to hold.  With three the kernel keeps within 168 registers, where the compiler spills a few that it
 // needs at the end; with 2 it uses 175.
 template <int HD, int NQ, bool PREFIX, int PER_SM>
@@ -767,7 +768,7 @@ __global__ void __launch_bounds__(kDecodeWarps * 32, PER_SM) attn_decode_int8_ke
 // results) finds its place by itself: nothing is handed out at run time and the result does not depend on timing.
 // The partial result of warp w for unit u goes to slot w + u: from one part of the row to the next w or u grows.
 // What bounds it: bytes; 11 us are spent around a stream that runs at the rate of a plain copy (1 x 8 kv heads x 4 queries: 131072
-// positions 53.2 us with the joining kernel, each further 131072 another 42.2).  A warp with a ring of its own, one CTA of 8 per SM:
+// positions 52.8 us with the joining kernel, each further 131072 another 42.2).  A warp with a ring of its own, one CTA of 8 per SM:
 // 201 KB of tiles under way, no barrier between warps.
 constexpr int kFlatWarpsPerSm = 8, kFlatWarps = kSms * kFlatWarpsPerSm;
 template <int HD, int NQ>
@@ -986,7 +987,7 @@ __global__ void __launch_bounds__((WIDE ? kJoinWarps : kWarps) * 32) attn_flat_j
 // the rows of a kv head being its queries (b, g) in the order b * G + g.  A warp carries 8 rows; the QW warps of a group
 // take the same tiles, which they fetch together into the group's ring, and the KW = 8 / QW groups take alternate tiles.
 // What bounds it: the s8 products of mma.sync, 8 cycles each on an SM's quarter, from 16 rows on (32 rows x 8 heads behind 16384
-// positions: 35.4 us with the decode behind it); below, start, digits and the hand-over (8 rows x 16 heads behind 2048: 11.4).
+// positions: 35.2 us with the decode behind it); below, start, digits and the hand-over (8 rows x 16 heads behind 2048: 11.4).
 template <int HD, int QW>
 struct PrefixShape {
     static constexpr int NQ = 8, KW = kWarps / QW;
